@@ -255,7 +255,7 @@ def _plain_tables(s):
 def _plain_store(s):
     case, slots, page = s["case"], s["slots"], s["case"]["page"]
     for x, cache, scale in ((s["k"], s["keys"], s["k_scale"]), (s["v"], s["values"], s["v_scale"])):
-        x = x.float() / scale
+        x = x.float() * (1 / scale)  # the reciprocal in 32 bits, then one product
         if case["cache"] == "e4m3":
             x = x.clamp(-448, 448)
         cache[slots // page, slots % page] = x.to(cache.dtype)
