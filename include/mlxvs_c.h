@@ -345,6 +345,157 @@ MLXVS_C_API int mlxvs_exchange_merge_device(
 MLXVS_C_API int mlxvs_exchange_destroy(void* exchange);
 
 /**
+ * Paged key-value cache: the operators of a language model's serving step
+ * next to the search.  No counterpart in the reference.  All pointers are
+ * device pointers; the calls enqueue work on stream and return without
+ * waiting, so a step of fixed sizes can be captured in a CUDA graph.
+ *
+ * A cache is `pages` pages of `page_size` rows (one row per token) for each
+ * of `heads` key heads.  A request's rows lie in the pages that its row of
+ * the page table lists, in order.  Tokens are rows of q / k / v; several may
+ * belong to one request (a prompt), each with the number of keys it sees.
+ */
+typedef enum {
+  MLXVS_FLOAT16 = 0,
+  MLXVS_BFLOAT16 = 1,
+  /** 8-bit cache rows: value = element * scale of the cache. */
+  MLXVS_FLOAT8_E4M3 = 2,
+} mlxvs_dtype;
+
+/** A cache's tensors; strides in elements, multiples of 16 bytes; the head
+ * dimension is contiguous, a multiple of 16 bytes and at most 256. */
+typedef struct {
+  void* keys;
+  void* values;
+  int64_t key_page_stride, key_row_stride, key_head_stride;
+  int64_t value_page_stride, value_row_stride, value_head_stride;
+  int64_t pages;
+  /** Bounds of the pages' keys, int8 [pages, heads, 2, dim] and float32
+   * [pages, heads], in the cache's units: codes[.., 0, d] * scale <= key[d]
+   * <= codes[.., 1, d] * scale.  May be NULL where no pages are selected. */
+  int8_t* codes;
+  float* scales;
+  int32_t page_size;
+  int32_t heads;
+  int32_t dim;
+  /** An mlxvs_dtype. */
+  int32_t type;
+  float key_scale;
+  float value_scale;
+} mlxvs_paged_cache;
+
+/** Queries of a step: q [tokens, heads, dim] (strides in elements, dim
+ * contiguous), the page table int32 [rows, width], each token's row of it
+ * (NULL: token t has row t) and how many keys the token sees (0: none). */
+typedef struct {
+  const void* q;
+  int64_t tokens;
+  int64_t token_stride, head_stride;
+  const int32_t* table;
+  int64_t rows, width;
+  const int32_t* requests;
+  const int32_t* lengths;
+  int32_t heads;
+  /** MLXVS_FLOAT16 or MLXVS_BFLOAT16. */
+  int32_t type;
+} mlxvs_paged_queries;
+
+/**
+ * Page tables and slot maps of one step.  Request r holds past[r] tokens and
+ * gets fresh[r] new ones; the pages it needs beyond the ceil(past / P) that
+ * its row of table [requests, width] lists are taken from free_pages, in
+ * request order, and entered in the table.  Per new token t of num_tokens
+ * (at least their number; the tokens past it are padding, so that a
+ * captured step can keep its size): token_requests (-1 for padding), lengths
+ * (the token's position + 1: the keys it sees; 0 for padding) and slots
+ * (page * page_size + row in the page, -1 where it gets none).  starts
+ * [requests + 1]: the requests' first tokens.  used[0]: pages asked of
+ * free_pages (the next step's list starts behind them), used[1]: new tokens
+ * that got no slot, because free_pages ended (their table entries are then
+ * -1), the table is too narrow, or a begun page is not in it.
+ */
+MLXVS_C_API int mlxvs_paged_tables_device(
+    const int32_t* past,
+    const int32_t* fresh,
+    int64_t requests,
+    int32_t page_size,
+    const int32_t* free_pages,
+    int64_t num_free,
+    int32_t* table,
+    int64_t width,
+    int64_t num_tokens,
+    int32_t* starts,
+    int32_t* token_requests,
+    int32_t* lengths,
+    int64_t* slots,
+    int32_t* used,
+    void* stream);
+
+/**
+ * Writes the rows k, v [tokens, heads, dim] (type MLXVS_FLOAT16 or
+ * MLXVS_BFLOAT16; strides in elements, multiples of 16 bytes) to their slots,
+ * times the float32 reciprocals of the cache's scales, rounded to its type
+ * (e4m3 saturates at 448); slots outside the cache are skipped.  Where the cache has codes and
+ * scales, the bounds of every page that got a row are made anew over its rows
+ * up to the last new one.  Slots must differ; a page's new rows come one
+ * after another, as mlxvs_paged_tables_device gives them.  NaN keys do not
+ * count in the bounds, infinite ones saturate.
+ */
+MLXVS_C_API int mlxvs_paged_store_device(
+    const mlxvs_paged_cache* cache,
+    const void* k,
+    const void* v,
+    int32_t type,
+    int64_t tokens,
+    int64_t k_token_stride,
+    int64_t k_head_stride,
+    int64_t v_token_stride,
+    int64_t v_head_stride,
+    const int64_t* slots,
+    void* stream);
+
+/**
+ * The n pages (positions in the request's row of the table, 1 <= n <= 256)
+ * that each token and key head attends to: pages int32 [tokens, heads, n] in
+ * ascending order, -1 past the last.  All pages that hold keys of the token
+ * when they are at most n; else the first `first` and last `last` of them and
+ * those of the best scores, ties to the lower page.  A page's score is an
+ * 8-bit upper bound of q . key over its rows, summed over the query heads of
+ * the key head, from the cache's codes and scales (keys and values are not
+ * read); it is exact in float32, so the choice is the same on every run.
+ */
+MLXVS_C_API int mlxvs_paged_select_device(
+    const mlxvs_paged_cache* cache,
+    const mlxvs_paged_queries* queries,
+    int32_t n,
+    int32_t first,
+    int32_t last,
+    int32_t* pages,
+    void* stream);
+
+/**
+ * Attention of each token and query head over the first lengths[t] keys of
+ * its request, or, with pages (as mlxvs_paged_select_device lists them, every
+ * page at most once), over those of them in the listed pages: softmax of
+ * scale * q . k, weighted sum of the values; out [tokens, query heads, dim]
+ * of q's type (contiguous) and, unless lse is NULL, the logarithm of the sum
+ * of exponentials, float32 [tokens, query heads].  Query head i reads key
+ * head i / (query heads / key heads).  A token with no keys (length 0, a
+ * request outside the table, only -1 pages) gets zeros and -inf; keys in
+ * pages outside the cache are left out.  Sums are float32, and joined in a
+ * fixed order: the same inputs give the same bits.
+ */
+MLXVS_C_API int mlxvs_paged_attention_device(
+    const mlxvs_paged_cache* cache,
+    const mlxvs_paged_queries* queries,
+    const int32_t* pages,
+    int32_t n,
+    float scale,
+    void* out,
+    float* lse,
+    void* stream);
+
+/**
  * Waits for stream and reports any error the library's kernels recorded on
  * the current device since the last call (a bounded wait that gave up).
  * Not in the reference (MLX reports errors at mx::eval).

@@ -6,6 +6,10 @@ of the reference):
     ids, distances = brute_force_knn(base, queries, k, metric="l2")
     ids, distances = hamming_knn(rows, queries, k)
 
+and the operators of a paged key-value cache that a serving step runs next to
+it (paged_tables, paged_store, paged_select, paged_attention: mlxvs_b200/
+paged.py).
+
 NumPy arrays (or anything array-like) go through the C API's host-memory
 entry points and come back as NumPy arrays; CUDA torch tensors stay on the
 device and come back as torch tensors on the same device, computed on the
@@ -38,6 +42,11 @@ __all__ = [
     "knn_keys",
     "hamming_keys",
     "merge_keys",
+    "PagedTables",
+    "paged_tables",
+    "paged_store",
+    "paged_select",
+    "paged_attention",
     "library_path",
     "version",
 ]
@@ -92,6 +101,10 @@ def _load():
         "mlxvs_exchange_keys": [p, ctypes.c_uint32, ctypes.POINTER(ctypes.c_void_p)],
         "mlxvs_exchange_merge_device": [p, ctypes.c_uint32, i64, i32, i32, p, i32, p, p, p],
         "mlxvs_exchange_destroy": [p],
+        "mlxvs_paged_tables_device": [p, p, i64, i32, p, i64, p, i64, i64, p, p, p, p, p, p],
+        "mlxvs_paged_store_device": [p, p, p, i32, i64, i64, i64, i64, i64, p, p],
+        "mlxvs_paged_select_device": [p, p, i32, i32, i32, p, p],
+        "mlxvs_paged_attention_device": [p, p, p, i32, ctypes.c_float, p, p, p],
         "mlxvs_device_synchronize": [p],
         "mlxvs_profile_enable": [i32],
         "mlxvs_profile_read": [ctypes.c_char_p, ctypes.POINTER(ctypes.c_double),
@@ -593,3 +606,12 @@ def profile_issued(kernel=None):
     name = kernel.encode() if kernel else None
     _check(_load().mlxvs_profile_issued(name, ctypes.byref(ops)))
     return ops.value
+
+
+from .paged import (  # noqa: E402  (it uses the helpers above)
+    PagedTables,
+    paged_attention,
+    paged_select,
+    paged_store,
+    paged_tables,
+)

@@ -14,9 +14,11 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmlxvs_b200.so")
-SOURCES = ["engine.cu", "c_api.cpp", "cpp_api.cu"]
+OBJECTS = os.path.join(HERE, "_build")
+SOURCES = ["engine.cu", "paged.cu", "c_api.cpp", "cpp_api.cu"]
 HEADERS = ["common.cuh", "gemm_topk.cuh", "gemm_topk_q.cuh", "hamming.cuh", "knn_kernels.cuh",
-           "select.cuh", "engine.h"]
+           "select.cuh", "engine.h", "host.h", "paged.h", "paged_common.cuh", "paged_tables.cuh",
+           "paged_store.cuh", "paged_select.cuh", "paged_attention.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -63,8 +65,20 @@ def build(verbose=False, force=False, extra=()):
     env = dict(os.environ)
     env.pop("NVCC_PREPEND_FLAGS", None)
     env.pop("NVCC_APPEND_FLAGS", None)
+    # One compiler per source, side by side, then one link.
+    os.makedirs(OBJECTS, exist_ok=True)
+    objects = [os.path.join(OBJECTS, f + ".o") for f in SOURCES]
+    running = []
+    for f, obj in zip(SOURCES, objects):
+        cmd = [nvcc, *flags(extra), "-c", "-o", obj, os.path.join(CSRC, f)]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        running.append((cmd, subprocess.Popen(cmd, env=env, cwd=CSRC)))
+    failed = [(cmd, p.returncode) for cmd, p in running if p.wait() != 0]
+    if failed:
+        raise subprocess.CalledProcessError(failed[0][1], failed[0][0])
     tmp = LIB + ".tmp"
-    cmd = [nvcc, *flags(extra), "-shared", "-o", tmp] + [os.path.join(CSRC, f) for f in SOURCES]
+    cmd = [nvcc, *ARCH, "-shared", "-o", tmp, *objects]
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True, env=env, cwd=CSRC)
@@ -75,9 +89,12 @@ def build(verbose=False, force=False, extra=()):
 def ptxas_report():
     """Registers / spills / shared memory per kernel (nvcc -Xptxas -v)."""
     nvcc = nvcc_path()
-    cmd = [nvcc, *flags(["-Xptxas", "-v"]), "-c", "-o", os.devnull, os.path.join(CSRC, "engine.cu")]
-    out = subprocess.run(cmd, capture_output=True, text=True, cwd=CSRC)
-    return out.stdout + out.stderr
+    report = ""
+    for source in ("engine.cu", "paged.cu"):
+        cmd = [nvcc, *flags(["-Xptxas", "-v"]), "-c", "-o", os.devnull, os.path.join(CSRC, source)]
+        out = subprocess.run(cmd, capture_output=True, text=True, cwd=CSRC)
+        report += out.stdout + out.stderr
+    return report
 
 
 if __name__ == "__main__":

@@ -12,6 +12,7 @@
 
 #include "engine.h"
 #include "mlxvs_c.h"
+#include "paged.h"
 
 namespace {
 
@@ -490,6 +491,50 @@ int mlxvs_hamming_knn_noalloc(const uint8_t* rows, int64_t n, const uint8_t* que
   return guarded([&] {
     mlxvs_b200::hamming_knn_noalloc(rows, n, queries, nq, bytes, k, ids, distances,
                                     static_cast<cudaStream_t>(stream));
+  });
+}
+
+int mlxvs_paged_tables_device(const int32_t* past, const int32_t* fresh, int64_t requests,
+                              int32_t page_size, const int32_t* free_pages, int64_t num_free,
+                              int32_t* table, int64_t width, int64_t num_tokens, int32_t* starts,
+                              int32_t* token_requests, int32_t* lengths, int64_t* slots,
+                              int32_t* used, void* stream) {
+  return guarded([&] {
+    mlxvs_b200::paged_tables(past, fresh, requests, page_size, free_pages, num_free, table, width,
+                             num_tokens, starts, token_requests, lengths, slots, used,
+                             static_cast<cudaStream_t>(stream));
+  });
+}
+
+int mlxvs_paged_store_device(const mlxvs_paged_cache* cache, const void* k, const void* v,
+                             int32_t type, int64_t tokens, int64_t k_token_stride,
+                             int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                             const int64_t* slots, void* stream) {
+  return guarded([&] {
+    require(cache != nullptr, "cache must not be NULL.");
+    mlxvs_b200::paged_store(*cache, k, v, type, tokens, k_token_stride, k_head_stride,
+                            v_token_stride, v_head_stride, slots,
+                            static_cast<cudaStream_t>(stream));
+  });
+}
+
+int mlxvs_paged_select_device(const mlxvs_paged_cache* cache, const mlxvs_paged_queries* queries,
+                              int32_t n, int32_t first, int32_t last, int32_t* pages,
+                              void* stream) {
+  return guarded([&] {
+    require(cache != nullptr && queries != nullptr, "cache and queries must not be NULL.");
+    mlxvs_b200::paged_select(*cache, *queries, n, first, last, pages,
+                             static_cast<cudaStream_t>(stream));
+  });
+}
+
+int mlxvs_paged_attention_device(const mlxvs_paged_cache* cache,
+                                 const mlxvs_paged_queries* queries, const int32_t* pages,
+                                 int32_t n, float scale, void* out, float* lse, void* stream) {
+  return guarded([&] {
+    require(cache != nullptr && queries != nullptr, "cache and queries must not be NULL.");
+    mlxvs_b200::paged_attention(*cache, *queries, pages, n, scale, out, lse,
+                                static_cast<cudaStream_t>(stream));
   });
 }
 

@@ -1,0 +1,209 @@
+// Host side of the paged key-value cache: argument checks and launches.
+#include "paged.h"
+
+#include <cmath>
+
+#include "host.h"
+#include "paged_attention.cuh"
+#include "paged_select.cuh"
+#include "paged_store.cuh"
+#include "paged_tables.cuh"
+
+namespace mlxvs_b200 {
+
+namespace {
+
+constexpr int MAX_DIM = 256;
+constexpr int MAX_PAGE = 1024;
+constexpr int MAX_SELECTED = 256;
+
+int type_size(int type) { return type == MLXVS_FLOAT8_E4M3 ? 1 : 2; }
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Calls f(T{}, C{}) with the element types of queries and cache.
+template <class F>
+void dispatch_types(int type, int cache_type, F&& f) {
+  if (type == MLXVS_FLOAT16 && cache_type == MLXVS_FLOAT16)
+    f(__half{}, __half{});
+  else if (type == MLXVS_FLOAT16)
+    f(__half{}, __nv_fp8_e4m3{});
+  else if (cache_type == MLXVS_BFLOAT16)
+    f(__nv_bfloat16{}, __nv_bfloat16{});
+  else
+    f(__nv_bfloat16{}, __nv_fp8_e4m3{});
+}
+
+void check_types(const std::string& op, int type, int cache_type) {
+  require(type == MLXVS_FLOAT16 || type == MLXVS_BFLOAT16,
+          op + "queries, keys and values must be float16 or bfloat16.");
+  require(cache_type == type || cache_type == MLXVS_FLOAT8_E4M3,
+          op + "the cache must have their type or be float8_e4m3.");
+}
+
+// Shape, strides and alignment of the cache's tensors.
+void check_cache(const std::string& op, const mlxvs_paged_cache& c, bool rows) {
+  require(c.pages >= 0 && c.pages < (1LL << 31), op + "the number of pages must be in [0, 2^31).");
+  require(c.page_size >= 1 && c.page_size <= MAX_PAGE, op + "page_size must be in [1, 1024].");
+  require(c.heads >= 1 && c.heads <= 65535, op + "the key heads must be in [1, 65535].");
+  const int unit = 16 / type_size(c.type);
+  const int d_unit = rows ? unit : 8;
+  require(c.dim >= d_unit && c.dim <= MAX_DIM && c.dim % d_unit == 0,
+          op + "the head dimension must be a multiple of " + std::to_string(d_unit) +
+              " and at most 256.");
+  if (!rows) return;
+  require(c.pages == 0 || (c.keys != nullptr && c.values != nullptr),
+          op + "keys and values must not be NULL.");
+  require(aligned16(c.keys) && aligned16(c.values),
+          op + "keys and values must be 16-byte aligned.");
+  for (int64_t s : {c.key_page_stride, c.key_row_stride, c.key_head_stride, c.value_page_stride,
+                    c.value_row_stride, c.value_head_stride})
+    require(s >= 0 && s % unit == 0,
+            op + "the cache's strides must be multiples of 16 bytes and not negative.");
+  require(std::isfinite(c.key_scale) && c.key_scale > 0 && std::isfinite(c.value_scale) &&
+              c.value_scale > 0,
+          op + "k_scale and v_scale must be positive and finite.");
+  require(std::isfinite(1.0f / c.key_scale) && std::isfinite(1.0f / c.value_scale),
+          op + "k_scale and v_scale must have finite reciprocals.");
+}
+
+void check_codes(const std::string& op, const mlxvs_paged_cache& c) {
+  require(c.codes != nullptr && c.scales != nullptr, op + "codes and scales must not be NULL.");
+  require(aligned16(c.codes), op + "codes must be 16-byte aligned.");
+}
+
+void check_queries(const std::string& op, const mlxvs_paged_cache& c,
+                   const mlxvs_paged_queries& q) {
+  check_types(op, q.type, c.type);
+  require(q.tokens >= 0 && q.tokens < (1LL << 31), op + "the tokens must be in [0, 2^31).");
+  require(q.heads >= 1 && q.heads % c.heads == 0 && q.heads / c.heads <= 128,
+          op + "the query heads must be 1 to 128 times the key heads.");
+  require(q.rows >= 0 && q.rows < (1LL << 31) && q.width >= 0 && q.width < (1LL << 31),
+          op + "the table must be int32 [requests, width].");
+  require(q.tokens == 0 || (q.q != nullptr && q.lengths != nullptr),
+          op + "q and lengths must not be NULL.");
+  require(q.table != nullptr || q.rows * q.width == 0, op + "table must not be NULL.");
+  require(q.requests != nullptr || q.tokens <= q.rows,
+          op + "without requests every token needs a row of the table.");
+  require(aligned16(q.q) && q.token_stride % 8 == 0 && q.head_stride % 8 == 0 &&
+              q.token_stride >= 0 && q.head_stride >= 0,
+          op + "q must be 16-byte aligned, with strides of multiples of 16 bytes.");
+}
+
+}  // namespace
+
+void paged_tables(const int32_t* past, const int32_t* fresh, int64_t requests, int page_size,
+                  const int32_t* free_pages, int64_t num_free, int32_t* table, int64_t width,
+                  int64_t num_tokens, int32_t* starts, int32_t* token_requests,
+                  int32_t* lengths, int64_t* slots, int32_t* used, cudaStream_t s) {
+  const std::string op = "[mlxvs::paged_tables] ";
+  require(requests >= 0 && requests < (1LL << 31), op + "the requests must be in [0, 2^31).");
+  require(page_size >= 1 && page_size <= MAX_PAGE, op + "page_size must be in [1, 1024].");
+  require(num_tokens >= 0 && num_tokens < (1LL << 31) - TABLES_TOKENS,
+          op + "num_tokens must be in [0, 2^31).");
+  require(num_free >= 0 && width >= 0 && width < (1LL << 31),
+          op + "the table must be int32 [requests, width].");
+  require(requests == 0 || (past != nullptr && fresh != nullptr),
+          op + "past and fresh must not be NULL.");
+  require(requests * width == 0 || table != nullptr, op + "table must not be NULL.");
+  require(num_free == 0 || free_pages != nullptr, op + "free_pages must not be NULL.");
+  require(starts != nullptr && used != nullptr &&
+              (num_tokens == 0 ||
+               (token_requests != nullptr && lengths != nullptr && slots != nullptr)),
+          op + "outputs must not be NULL.");
+  device_info();
+  const TablesParams p{past,  fresh,      requests, FastDiv((uint32_t)page_size), free_pages,
+                       num_free, table,  width,    num_tokens, starts, token_requests,
+                       lengths, slots, used};
+  const unsigned blocks =
+      (unsigned)std::max<int64_t>(1, (num_tokens + TABLES_TOKENS - 1) / TABLES_TOKENS);
+  ProfScope prof("paged_tables", s);
+  paged_tables_kernel<<<blocks, TABLES_THREADS, 0, s>>>(p);
+  CK(cudaGetLastError());
+}
+
+void paged_store(const mlxvs_paged_cache& c, const void* k, const void* v, int type,
+                 int64_t tokens, int64_t k_token, int64_t k_head, int64_t v_token,
+                 int64_t v_head, const int64_t* slots, cudaStream_t s) {
+  const std::string op = "[mlxvs::paged_store] ";
+  check_types(op, type, c.type);
+  check_cache(op, c, true);
+  require(tokens >= 0 && tokens < (1LL << 31), op + "the tokens must be in [0, 2^31).");
+  require(tokens == 0 || (k != nullptr && v != nullptr && slots != nullptr),
+          op + "k, v and slots must not be NULL.");
+  require(aligned16(k) && aligned16(v), op + "k and v must be 16-byte aligned.");
+  for (int64_t x : {k_token, k_head, v_token, v_head})
+    require(x >= 0 && x % 8 == 0, op + "the strides of k and v must be multiples of 16 bytes.");
+  if (c.codes != nullptr || c.scales != nullptr) check_codes(op, c);
+  device_info();
+  if (tokens == 0 || c.pages == 0) return;
+  StoreParams p{k, v, tokens, k_token, k_head, v_token, v_head, slots, c.keys, c.values,
+                c.key_page_stride, c.key_row_stride, c.key_head_stride,
+                c.value_page_stride, c.value_row_stride, c.value_head_stride,
+                c.pages, FastDiv((uint32_t)c.page_size), c.heads, c.dim,
+                1.0f / c.key_scale, 1.0f / c.value_scale, c.codes, c.scales};
+  ProfScope prof("paged_store", s);
+  dispatch_types(type, c.type, [&](auto t, auto ct) {
+    paged_store_kernel<decltype(t), decltype(ct)><<<(unsigned)tokens, 256, 0, s>>>(p);
+  });
+  CK(cudaGetLastError());
+}
+
+void paged_select(const mlxvs_paged_cache& c, const mlxvs_paged_queries& q, int n, int first,
+                  int last, int32_t* pages, cudaStream_t s) {
+  const std::string op = "[mlxvs::paged_select] ";
+  check_cache(op, c, false);
+  check_codes(op, c);
+  check_queries(op, c, q);
+  require(n >= 1 && n <= MAX_SELECTED, op + "n must be in [1, 256].");
+  require(first >= 0 && last >= 0 && first + last <= n,
+          op + "first and last must be at least 0 and together at most n.");
+  require(q.tokens == 0 || pages != nullptr, op + "pages must not be NULL.");
+  DeviceInfo& dev = device_info();
+  const size_t smem = (size_t)q.width * 4;
+  require(smem + 8192 <= (size_t)dev.max_smem,
+          op + "the table must have at most " + std::to_string((dev.max_smem - 8192) / 4) +
+              " pages a request.");
+  if (q.tokens == 0) return;
+  int shift = 0;
+  while ((1 << shift) < q.heads / c.heads) ++shift;
+  const SelectParams p{q.q, q.tokens, q.token_stride, q.head_stride, c.heads,
+                       q.heads / c.heads, c.dim, shift, c.codes, c.scales, c.pages, q.table,
+                       q.rows, q.width, q.requests, q.lengths, FastDiv((uint32_t)c.page_size),
+                       n, first, last, pages};
+  ProfScope prof("paged_select", s);
+  dispatch_types(q.type, q.type, [&](auto t, auto) {
+    auto* kernel = paged_select_kernel<decltype(t)>;
+    CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    kernel<<<dim3((unsigned)q.tokens, c.heads), SELECT_THREADS, smem, s>>>(p);
+  });
+  CK(cudaGetLastError());
+}
+
+void paged_attention(const mlxvs_paged_cache& c, const mlxvs_paged_queries& q,
+                     const int32_t* pages, int n, float scale, void* out, float* lse,
+                     cudaStream_t s) {
+  const std::string op = "[mlxvs::paged_attention] ";
+  check_cache(op, c, true);
+  check_queries(op, c, q);
+  require(pages == nullptr || n >= 1, op + "pages must be int32 [tokens, key heads, n].");
+  require(std::isfinite(scale), op + "scale must be finite.");
+  require(q.tokens == 0 || out != nullptr, op + "out must not be NULL.");
+  require(aligned16(out), op + "out must be 16-byte aligned.");
+  device_info();
+  if (q.tokens == 0) return;
+  AttentionParams p{q.q, q.tokens, q.token_stride, q.head_stride, c.heads, q.heads / c.heads,
+                    c.dim, c.keys, c.values, c.key_page_stride, c.key_row_stride,
+                    c.key_head_stride, c.value_page_stride, c.value_row_stride,
+                    c.value_head_stride, c.pages, FastDiv((uint32_t)c.page_size), q.table,
+                    q.rows, q.width, q.requests, q.lengths, pages, n, scale * c.key_scale,
+                    c.value_scale, out, lse};
+  ProfScope prof("paged_attention", s);
+  dispatch_types(q.type, c.type, [&](auto t, auto ct) {
+    paged_attention_kernel<decltype(t), decltype(ct)>
+        <<<dim3((unsigned)q.tokens, q.heads), ATTENTION_WARPS * 32, 0, s>>>(p);
+  });
+  CK(cudaGetLastError());
+}
+
+}  // namespace mlxvs_b200
