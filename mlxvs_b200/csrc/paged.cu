@@ -2,6 +2,7 @@
 #include "paged.h"
 
 #include <cmath>
+#include <type_traits>
 
 #include "host.h"
 #include "paged_attention.cuh"
@@ -88,6 +89,35 @@ void check_queries(const std::string& op, const mlxvs_paged_cache& c,
   require(aligned16(q.q) && q.token_stride % 8 == 0 && q.head_stride % 8 == 0 &&
               q.token_stride >= 0 && q.head_stride >= 0,
           op + "q must be 16-byte aligned, with strides of multiples of 16 bytes.");
+}
+
+// The attention kernel on every SM and, when it may have cut rows, the kernel
+// that joins them, launched so that it is ready when the first one ends.
+template <class T, class C, int DP, int NT>
+void launch_attention(AttentionParams p, DeviceInfo& dev, Scratch& scratch, cudaStream_t s) {
+  using S = AttentionShape<T, C, DP, NT>;
+  const int blocks = dev.sms * S::BLOCKS;
+  p.part = scratch.alloc<float>((size_t)blocks * 2 * S::PART);
+  p.cut = scratch.alloc<int4>(blocks);
+  auto* kernel = p.selected ? paged_attention_kernel<T, C, DP, NT, true>
+                            : paged_attention_kernel<T, C, DP, NT, false>;
+  CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+  {
+    ProfScope prof("paged_attention", s);
+    kernel<<<blocks, S::WARPS * 32, S::SMEM, s>>>(p);
+    CK(cudaGetLastError());
+  }
+  ProfScope prof("paged_attention_join", s);
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(blocks, std::min(p.group, S::HEADS));
+  config.blockDim = dim3(DP);
+  config.stream = s;
+  cudaLaunchAttribute attribute;
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  CK(cudaLaunchKernelEx(&config, paged_attention_join_kernel<T, DP, NT>, p));
 }
 
 }  // namespace
@@ -186,24 +216,34 @@ void paged_attention(const mlxvs_paged_cache& c, const mlxvs_paged_queries& q,
   const std::string op = "[mlxvs::paged_attention] ";
   check_cache(op, c, true);
   check_queries(op, c, q);
-  require(pages == nullptr || n >= 1, op + "pages must be int32 [tokens, key heads, n].");
+  require(pages == nullptr || (n >= 1 && n <= (1 << 20)),
+          op + "pages must be int32 [tokens, key heads, n], n at most 2^20.");
   require(std::isfinite(scale), op + "scale must be finite.");
   require(q.tokens == 0 || out != nullptr, op + "out must not be NULL.");
   require(aligned16(out), op + "out must be 16-byte aligned.");
-  device_info();
+  DeviceInfo& dev = device_info();
   if (q.tokens == 0) return;
+  const float log2e = 1.44269504088896f;
   AttentionParams p{q.q, q.tokens, q.token_stride, q.head_stride, c.heads, q.heads / c.heads,
                     c.dim, c.keys, c.values, c.key_page_stride, c.key_row_stride,
                     c.key_head_stride, c.value_page_stride, c.value_row_stride,
                     c.value_head_stride, c.pages, FastDiv((uint32_t)c.page_size), q.table,
-                    q.rows, q.width, q.requests, q.lengths, pages, n, scale * c.key_scale,
-                    c.value_scale, out, lse};
-  ProfScope prof("paged_attention", s);
+                    q.rows, q.width, q.requests, q.lengths, pages, n, scale * c.key_scale * log2e,
+                    c.value_scale, out, lse, nullptr, nullptr};
+  Scratch scratch(s);
   dispatch_types(q.type, c.type, [&](auto t, auto ct) {
-    paged_attention_kernel<decltype(t), decltype(ct)>
-        <<<dim3((unsigned)q.tokens, q.heads), ATTENTION_WARPS * 32, 0, s>>>(p);
+    auto shaped = [&](auto dp, auto nt) {
+      launch_attention<decltype(t), decltype(ct), decltype(dp)::value, decltype(nt)::value>(
+          p, dev, scratch, s);
+    };
+    auto wide = [&](auto dp) {
+      if (p.group <= 8) shaped(dp, std::integral_constant<int, 1>{});
+      else shaped(dp, std::integral_constant<int, 2>{});
+    };
+    if (p.dim <= 64) wide(std::integral_constant<int, 64>{});
+    else if (p.dim <= 128) wide(std::integral_constant<int, 128>{});
+    else wide(std::integral_constant<int, 256>{});
   });
-  CK(cudaGetLastError());
 }
 
 }  // namespace mlxvs_b200
