@@ -91,6 +91,13 @@ void check_queries(const std::string& op, const mlxvs_paged_cache& c,
           op + "q must be 16-byte aligned, with strides of multiples of 16 bytes.");
 }
 
+// More than 48 KB of dynamic shared memory has to be asked for.
+template <class K>
+void allow_smem(K* kernel, size_t bytes) {
+  if (bytes > 40 * 1024)
+    CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+}
+
 // The attention kernel on every SM and, when it may have cut rows, the kernel
 // that joins them, launched so that it is ready when the first one ends.
 template <class T, class C, int DP, int NT>
@@ -101,7 +108,7 @@ void launch_attention(AttentionParams p, DeviceInfo& dev, Scratch& scratch, cuda
   p.cut = scratch.alloc<int4>(blocks);
   auto* kernel = p.selected ? paged_attention_kernel<T, C, DP, NT, true>
                             : paged_attention_kernel<T, C, DP, NT, false>;
-  CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+  allow_smem(kernel, S::SMEM);
   {
     ProfScope prof("paged_attention", s);
     kernel<<<blocks, S::WARPS * 32, S::SMEM, s>>>(p);
@@ -190,10 +197,10 @@ void paged_select(const mlxvs_paged_cache& c, const mlxvs_paged_queries& q, int 
           op + "first and last must be at least 0 and together at most n.");
   require(q.tokens == 0 || pages != nullptr, op + "pages must not be NULL.");
   DeviceInfo& dev = device_info();
-  const size_t smem = (size_t)q.width * 4;
-  require(smem + 8192 <= (size_t)dev.max_smem,
-          op + "the table must have at most " + std::to_string((dev.max_smem - 8192) / 4) +
-              " pages a request.");
+  // keys of one token and the static arrays must fit a block's shared memory
+  const int64_t room = (dev.max_smem - 16384) / 4;
+  require(q.width <= room,
+          op + "the table must have at most " + std::to_string(room) + " pages a request.");
   if (q.tokens == 0) return;
   int shift = 0;
   while ((1 << shift) < q.heads / c.heads) ++shift;
@@ -201,13 +208,33 @@ void paged_select(const mlxvs_paged_cache& c, const mlxvs_paged_queries& q, int 
                        q.heads / c.heads, c.dim, shift, c.codes, c.scales, c.pages, q.table,
                        q.rows, q.width, q.requests, q.lengths, FastDiv((uint32_t)c.page_size),
                        n, first, last, pages};
+  // Prompts (more tokens than requests) share the pages' codes between 8 tokens
+  // of a tile; single tokens have pages of their own.  Clusters share the pages
+  // of few tiles among more SMs.
+  const bool tiles = q.tokens > q.rows && 8 * q.width <= room;
+  const int64_t units = (q.tokens + (tiles ? 7 : 0)) / (tiles ? 8 : 1);
+  int cluster = 1;
+  while (cluster < 8 && units * c.heads * cluster < dev.sms && cluster * 128 < q.width)
+    cluster *= 2;
   ProfScope prof("paged_select", s);
   dispatch_types(q.type, q.type, [&](auto t, auto) {
-    auto* kernel = paged_select_kernel<decltype(t)>;
-    CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    kernel<<<dim3((unsigned)q.tokens, c.heads), SELECT_THREADS, smem, s>>>(p);
+    using T = decltype(t);
+    auto* kernel = tiles ? paged_select_kernel<T, 8> : paged_select_kernel<T, 1>;
+    const size_t smem = (size_t)(tiles ? 8 : 1) * q.width * 4;
+    allow_smem(kernel, smem);
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)(units * cluster), c.heads);
+    config.blockDim = dim3(SELECT_WARPS * 32);
+    config.dynamicSmemBytes = smem;
+    config.stream = s;
+    cudaLaunchAttribute attribute;
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = cluster;
+    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    CK(cudaLaunchKernelEx(&config, kernel, p));
   });
-  CK(cudaGetLastError());
 }
 
 void paged_attention(const mlxvs_paged_cache& c, const mlxvs_paged_queries& q,
