@@ -172,16 +172,28 @@ void paged_store(const mlxvs_paged_cache& c, const void* k, const void* v, int t
   for (int64_t x : {k_token, k_head, v_token, v_head})
     require(x >= 0 && x % 8 == 0, op + "the strides of k and v must be multiples of 16 bytes.");
   if (c.codes != nullptr || c.scales != nullptr) check_codes(op, c);
-  device_info();
+  DeviceInfo& dev = device_info();
   if (tokens == 0 || c.pages == 0) return;
   StoreParams p{k, v, tokens, k_token, k_head, v_token, v_head, slots, c.keys, c.values,
                 c.key_page_stride, c.key_row_stride, c.key_head_stride,
                 c.value_page_stride, c.value_row_stride, c.value_head_stride,
                 c.pages, FastDiv((uint32_t)c.page_size), c.heads, c.dim,
                 1.0f / c.key_scale, 1.0f / c.value_scale, c.codes, c.scales};
+  // Chunks of one token while that fills the GPU (single tokens end a page's
+  // rows each, so a chunk of them would go one after another), 32 at most.
+  const int64_t chunk =
+      std::max<int64_t>(1, std::min<int64_t>(32, tokens * c.heads / (dev.sms * 16)));
+  const dim3 grid((unsigned)((tokens + chunk - 1) / chunk),
+                  (c.heads + STORE_WARPS - 1) / STORE_WARPS);
   ProfScope prof("paged_store", s);
   dispatch_types(type, c.type, [&](auto t, auto ct) {
-    paged_store_kernel<decltype(t), decltype(ct)><<<(unsigned)tokens, 256, 0, s>>>(p);
+    auto lanes = [&](auto n) {
+      paged_store_kernel<decltype(t), decltype(ct), decltype(n)::value>
+          <<<grid, STORE_WARPS * 32, 0, s>>>(p, (int)chunk);
+    };
+    if (c.dim <= 64) lanes(std::integral_constant<int, 8>{});
+    else if (c.dim <= 128) lanes(std::integral_constant<int, 16>{});
+    else lanes(std::integral_constant<int, 32>{});
   });
   CK(cudaGetLastError());
 }

@@ -10,6 +10,8 @@
 // alone: storing a page in one step or row by row gives the same bits.
 #pragma once
 
+#include <type_traits>
+
 #include "paged_common.cuh"
 
 namespace mlxvs_b200 {
@@ -29,65 +31,146 @@ struct StoreParams {
   float* scales;   // [pages, heads]
 };
 
-// One block per token.  The block of the last new row of a page reads the
-// page's rows back (the earlier new ones from the input, since other blocks
-// write them) and makes its bounds, one warp per key head.
-template <class T, class C>
-__global__ void __launch_bounds__(256) paged_store_kernel(const StoreParams p) {
-  const int64_t t = blockIdx.x;
-  const int64_t slot = p.slots[t];
+constexpr int STORE_WARPS = 8;
+
+template <class T>
+struct alignas(sizeof(T) * 8) Eight {
+  T x[8];
+};
+
+// One warp per key head and chunk of up to 32 tokens, LANES lanes per row (8
+// channels each, so 16-byte loads), ROWS rows side by side.  First it copies
+// the chunk's rows; then, for each page whose last new row lies in the chunk,
+// it reads the page's rows (the new ones from the input, which other warps may
+// still be writing to the cache, the older ones from the cache) and makes its
+// bounds.  The second reading of new rows hits L2.
+//
+// Bound: the copies by HBM; single tokens by the latency of slot -> rows of
+// the page -> codes.
+template <class T, class C, int LANES>
+__global__ void __launch_bounds__(STORE_WARPS * 32)
+    paged_store_kernel(const StoreParams p, const int chunk) {
+  constexpr int ROWS = 32 / LANES;
+  const int lane = threadIdx.x & 31, sub = lane / LANES, d = (lane % LANES) * 8;
+  const int h = blockIdx.y * STORE_WARPS + (threadIdx.x >> 5);
+  if (h >= p.heads) return;
+  const bool mine = d < p.dim;
   const int64_t P = p.page.d;
-  if (slot < 0 || slot >= p.pages * P) return;
-  const int64_t page = slot / P, row = slot % P;
-  const T* k = static_cast<const T*>(p.k);
-  const T* v = static_cast<const T*>(p.v);
-  C* keys = static_cast<C*>(p.keys);
-  C* values = static_cast<C*>(p.values);
-  for (int i = threadIdx.x; i < p.heads * p.dim; i += blockDim.x) {
-    const int h = i / p.dim, d = i % p.dim;
-    keys[page * p.key_page + row * p.key_row + h * p.key_head + d] =
-        from_float<C>(to_float(k[t * p.k_token + h * p.k_head + d]) * p.k_inverse);
-    values[page * p.value_page + row * p.value_row + h * p.value_head + d] =
-        from_float<C>(to_float(v[t * p.v_token + h * p.v_head + d]) * p.v_inverse);
+  const int64_t t0 = (int64_t)blockIdx.x * chunk;
+  const int count = (int)min((int64_t)chunk, p.tokens - t0);
+  const T* k = static_cast<const T*>(p.k) + h * p.k_head + d;
+  const T* v = static_cast<const T*>(p.v) + h * p.v_head + d;
+  C* keys = static_cast<C*>(p.keys) + h * p.key_head + d;
+  C* values = static_cast<C*>(p.values) + h * p.value_head + d;
+
+  // one token per lane: its page and row, and whether it is its page's last
+  int64_t slot = -1, page = -1;
+  int row = 0;
+  bool last = false;
+  if (lane < count) {
+    slot = p.slots[t0 + lane];
+    if (slot >= 0 && slot < p.pages * P) {
+      page = slot / P, row = (int)(slot - page * P);
+      last = !(row + 1 < P && t0 + lane + 1 < p.tokens && p.slots[t0 + lane + 1] == slot + 1);
+    }
+  }
+  auto rounded = [](const Eight<T>& x, float by) {
+    Eight<C> y;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      y.x[i] = std::is_same<T, C>::value && by == 1.0f
+                   ? *reinterpret_cast<const C*>(&x.x[i])
+                   : from_float<C>(to_float(x.x[i]) * by);
+    return y;
+  };
+  constexpr int UNROLL = 4;
+  for (int i0 = 0; i0 < count; i0 += ROWS * UNROLL) {
+    Eight<T> kx[UNROLL], vx[UNROLL];
+    int64_t pg[UNROLL];
+    int r[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int i = i0 + u * ROWS + sub;
+      pg[u] = __shfl_sync(~0u, page, i & 31), r[u] = __shfl_sync(~0u, row, i & 31);
+      if (i >= count || !mine) pg[u] = -1;
+      if (pg[u] >= 0) {
+        kx[u] = *reinterpret_cast<const Eight<T>*>(k + (t0 + i) * p.k_token);
+        vx[u] = *reinterpret_cast<const Eight<T>*>(v + (t0 + i) * p.v_token);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if (pg[u] >= 0) {
+        *reinterpret_cast<Eight<C>*>(keys + pg[u] * p.key_page + r[u] * p.key_row) =
+            rounded(kx[u], p.k_inverse);
+        *reinterpret_cast<Eight<C>*>(values + pg[u] * p.value_page + r[u] * p.value_row) =
+            rounded(vx[u], p.v_inverse);
+      }
   }
   if (p.codes == nullptr) return;
-  if (t + 1 < p.tokens && p.slots[t + 1] == slot + 1 && row + 1 < P) return;
-  int64_t fresh = 1;  // new rows of this page: the tokens t - fresh + 1 .. t
-  while (fresh <= row && fresh <= t && p.slots[t - fresh] == slot - fresh) ++fresh;
-  const int lane = threadIdx.x & 31;
-  for (int h = threadIdx.x >> 5; h < p.heads; h += blockDim.x >> 5) {
-    float lo[8], hi[8], top = 0.0f;
+
+  for (uint32_t ends = __ballot_sync(~0u, last); ends != 0; ends &= ends - 1) {
+    const int e = __ffs(ends) - 1;
+    const int64_t te = t0 + e;
+    const int64_t pg = __shfl_sync(~0u, page, e), se = __shfl_sync(~0u, slot, e);
+    const int re = __shfl_sync(~0u, row, e);
+    // the page's first new row: its new rows are the tokens te, te - 1, ...
+    int begin = re;
+    while (begin > 0) {
+      const int back = re - begin + 1 + lane;  // this lane's row is re - back
+      const bool fresh = back <= re && back <= te && p.slots[te - back] == se - back;
+      const uint32_t all = __ballot_sync(~0u, fresh);
+      const int run = all == ~0u ? 32 : __ffs(~all) - 1;
+      begin -= run;
+      if (run < 32) break;
+    }
+    float lo[8], hi[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int d = lane + 32 * j;
-      lo[j] = INFINITY, hi[j] = -INFINITY;
-      if (d >= p.dim) continue;
-      for (int64_t r = 0; r <= row; ++r) {
-        const int64_t back = row - r;
-        float x;
-        if (back < fresh)
-          x = to_float(from_float<C>(to_float(k[(t - back) * p.k_token + h * p.k_head + d]) *
-                                     p.k_inverse));
-        else
-          x = to_float(keys[page * p.key_page + r * p.key_row + h * p.key_head + d]);
-        lo[j] = fminf(lo[j], x), hi[j] = fmaxf(hi[j], x);
+    for (int i = 0; i < 8; ++i) lo[i] = INFINITY, hi[i] = -INFINITY;
+    auto take = [&](const Eight<C>& x) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float y = to_float(x.x[i]);  // fminf and fmaxf pass over NaN
+        lo[i] = fminf(lo[i], y), hi[i] = fmaxf(hi[i], y);
       }
-      if (lo[j] > hi[j]) lo[j] = hi[j] = 0.0f;  // nothing but NaN
-      top = fmaxf(top, fmaxf(fabsf(lo[j]), fabsf(hi[j])));
+    };
+    if (mine) {
+      const C* old = keys + pg * p.key_page;
+#pragma unroll 8
+      for (int r = sub; r < begin; r += ROWS)
+        take(*reinterpret_cast<const Eight<C>*>(old + r * p.key_row));
+#pragma unroll 4
+      for (int r = begin + sub; r <= re; r += ROWS)
+        take(rounded(*reinterpret_cast<const Eight<T>*>(k + (te - (re - r)) * p.k_token),
+                     p.k_inverse));
+    }
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+#pragma unroll
+      for (int o = LANES; o < 32; o <<= 1) {
+        lo[i] = fminf(lo[i], __shfl_xor_sync(~0u, lo[i], o));
+        hi[i] = fmaxf(hi[i], __shfl_xor_sync(~0u, hi[i], o));
+      }
+      if (lo[i] > hi[i]) lo[i] = hi[i] = 0.0f;  // nothing but NaN
+      top = fmaxf(top, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-    const int e = code_exponent(top);
-    const float by = exp2_int(e);
-    int8_t* codes = p.codes + ((page * p.heads + h) * 2) * p.dim;
+    for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+    const int x = code_exponent(top);
+    const float by = exp2_int(x);
+    if (mine && sub == 0) {
+      Eight<int8_t> a, b;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int d = lane + 32 * j;
-      if (d >= p.dim) continue;
-      codes[d] = (int8_t)fmaxf(fminf(floorf(lo[j] * by), 127.0f), -127.0f);
-      codes[p.dim + d] = (int8_t)fminf(fmaxf(ceilf(hi[j] * by), -127.0f), 127.0f);
+      for (int i = 0; i < 8; ++i) {
+        a.x[i] = (int8_t)fmaxf(fminf(floorf(lo[i] * by), 127.0f), -127.0f);
+        b.x[i] = (int8_t)fminf(fmaxf(ceilf(hi[i] * by), -127.0f), 127.0f);
+      }
+      int8_t* codes = p.codes + ((pg * p.heads + h) * 2) * p.dim + d;
+      *reinterpret_cast<Eight<int8_t>*>(codes) = a;
+      *reinterpret_cast<Eight<int8_t>*>(codes + p.dim) = b;
     }
-    if (lane == 0) p.scales[page * p.heads + h] = exp2_int(-e);
+    if (lane == 0) p.scales[pg * p.heads + h] = exp2_int(-x);
   }
 }
 

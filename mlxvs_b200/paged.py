@@ -44,12 +44,11 @@ def _type(t, op, name):
 
 def _want(t, op, name, dtype, dim, device):
     """A contiguous CUDA tensor of the given type and number of dimensions."""
-    if not (_is_torch(t) and t.is_cuda and t.dtype == dtype and t.dim() == dim
-            and t.is_contiguous()):
+    if not (_is_torch(t) and t.dtype is dtype and t.dim() == dim and t.is_contiguous()
+            and t.is_cuda):
         raise ValueError(f"[{op}] {name} must be a contiguous {dim}-D CUDA tensor of {dtype}.")
     if t.device != device:
         raise ValueError(f"[{op}] {name} must be on {device}.")
-    return t
 
 
 def _rows(t, op, name, dims):
