@@ -104,8 +104,8 @@ template <class T, class C, int DP, int NT>
 void launch_attention(AttentionParams p, DeviceInfo& dev, Scratch& scratch, cudaStream_t s) {
   using S = AttentionShape<T, C, DP, NT>;
   const int blocks = dev.sms * S::BLOCKS;
-  p.part = scratch.alloc<float>((size_t)blocks * 2 * S::PART);
-  p.cut = scratch.alloc<int4>(blocks);
+  p.cut = scratch.alloc<int4>(blocks + ((size_t)blocks * 2 * S::PART + 3) / 4);
+  p.part = reinterpret_cast<float*>(p.cut + blocks);
   auto* kernel = p.selected ? paged_attention_kernel<T, C, DP, NT, true>
                             : paged_attention_kernel<T, C, DP, NT, false>;
   allow_smem(kernel, S::SMEM);

@@ -19,7 +19,9 @@ for the GPU, so a step of fixed sizes can be captured in a CUDA graph.
 import collections
 import struct
 
-from . import _check, _is_torch, _load, _stream_handle, _torch
+import torch
+
+from . import _check, _load
 
 PagedTables = collections.namedtuple("PagedTables", "starts requests lengths slots used")
 
@@ -27,101 +29,112 @@ PagedTables = collections.namedtuple("PagedTables", "starts requests lengths slo
 _CACHE = struct.Struct("=QQqqqqqqqQQiiiiff")
 _QUERIES = struct.Struct("=QqqqQqqQQii")
 
-_types = None
+_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float8_e4m3fn: 2}
+
+# A decoding step makes these calls per layer, so their own time counts: the
+# checks below read each tensor's fields once, and the stream is read without
+# the Stream object that torch.cuda.current_stream builds.
+_current_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch.cuda.current_device
 
 
 def _type(t, op, name):
-    global _types
-    if _types is None:
-        torch = _torch()
-        _types = {torch.float16: 0, torch.bfloat16: 1, torch.float8_e4m3fn: 2}
-    try:
-        return _types[t.dtype]
-    except KeyError:
+    code = _TYPES.get(t.dtype)
+    if code is None:
         raise ValueError(f"[{op}] {name} must be float16, bfloat16 or, in a cache, "
-                         f"float8_e4m3fn; got {t.dtype}.") from None
+                         f"float8_e4m3fn; got {t.dtype}.")
+    return code
 
 
-def _want(t, op, name, dtype, dim, device):
-    """A contiguous CUDA tensor of the given type and number of dimensions."""
-    if not (_is_torch(t) and t.dtype is dtype and t.dim() == dim and t.is_contiguous()
-            and t.is_cuda):
+def _want(t, op, name, dtype, dim, index):
+    """Checks for a contiguous tensor of the given type and number of
+    dimensions on the CUDA device `index`."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.dim() == dim
+            and t.is_contiguous() and t.is_cuda):
         raise ValueError(f"[{op}] {name} must be a contiguous {dim}-D CUDA tensor of {dtype}.")
-    if t.device != device:
-        raise ValueError(f"[{op}] {name} must be on {device}.")
+    if t.get_device() != index:
+        raise ValueError(f"[{op}] {name} must be on cuda:{index}.")
 
 
 def _rows(t, op, name, dims):
-    """A CUDA tensor with a contiguous last dimension."""
-    if not (_is_torch(t) and t.is_cuda and t.dim() == len(dims)):
+    """The strides of a CUDA tensor with a contiguous last dimension."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == len(dims)):
         raise ValueError(f"[{op}] {name} must be a CUDA tensor [{', '.join(dims)}].")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    strides = t.stride()
+    if strides[-1] != 1 and t.shape[-1] > 1:
         raise ValueError(f"[{op}] {name} must be contiguous in its last dimension.")
-    return t
+    return strides
 
 
-def _bounds(codes, scales, op, pages, heads, dim, device):
-    torch = _torch()
-    _want(codes, op, "codes", torch.int8, 4, device)
-    _want(scales, op, "scales", torch.float32, 2, device)
-    if tuple(codes.shape) != (pages, heads, 2, dim) or tuple(scales.shape) != (pages, heads):
+def _bounds(codes, scales, op, pages, heads, dim, index):
+    _want(codes, op, "codes", torch.int8, 4, index)
+    _want(scales, op, "scales", torch.float32, 2, index)
+    if codes.shape != (pages, heads, 2, dim) or scales.shape != (pages, heads):
         raise ValueError(f"[{op}] codes must be [pages, key heads, 2, dim] and scales "
                          "[pages, key heads].")
 
 
-def _cache(keys, values, codes, scales, k_scale, v_scale, op, device):
-    _rows(keys, op, "keys", ("pages", "page_size", "key heads", "dim"))
-    _rows(values, op, "values", ("pages", "page_size", "key heads", "dim"))
-    if keys.shape != values.shape or keys.dtype != values.dtype:
+_CACHE_DIMS = ("pages", "page_size", "key heads", "dim")
+_Q_DIMS = ("tokens", "query heads", "dim")
+_K_DIMS = ("tokens", "key heads", "dim")
+
+
+def _cache(keys, values, codes, scales, k_scale, v_scale, op, index):
+    """mlxvs_paged_cache of the tensors, and their shape."""
+    ks = _rows(keys, op, "keys", _CACHE_DIMS)
+    vs = _rows(values, op, "values", _CACHE_DIMS)
+    shape = keys.shape
+    if values.shape != shape or keys.dtype is not values.dtype:
         raise ValueError(f"[{op}] keys and values must have the same shape and type.")
-    if keys.device != device or values.device != device:
-        raise ValueError(f"[{op}] keys and values must be on {device}.")
-    pages, page_size, heads, dim = keys.shape
+    if keys.get_device() != index or values.get_device() != index:
+        raise ValueError(f"[{op}] keys and values must be on cuda:{index}.")
+    pages, page_size, heads, dim = shape
+    at_codes = at_scales = 0
     if codes is not None or scales is not None:
-        _bounds(codes, scales, op, pages, heads, dim, device)
-    ks, vs = keys.stride(), values.stride()
+        _bounds(codes, scales, op, pages, heads, dim, index)
+        at_codes, at_scales = codes.data_ptr(), scales.data_ptr()
     return _CACHE.pack(
         keys.data_ptr(), values.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], pages,
-        codes.data_ptr() if codes is not None else 0,
-        scales.data_ptr() if scales is not None else 0,
-        page_size, heads, dim, _type(keys, op, "keys"), k_scale, v_scale)
+        at_codes, at_scales, page_size, heads, dim, _type(keys, op, "keys"), k_scale,
+        v_scale), shape
 
 
 def _queries(q, table, lengths, requests, op):
-    torch = _torch()
-    _rows(q, op, "q", ("tokens", "query heads", "dim"))
-    device = q.device
-    _want(table, op, "table", torch.int32, 2, device)
-    _want(lengths, op, "lengths", torch.int32, 1, device)
-    tokens, heads, _ = q.shape
+    """mlxvs_paged_queries of the tensors, q's shape and its device."""
+    qs = _rows(q, op, "q", _Q_DIMS)
+    index = q.get_device()
+    _want(table, op, "table", torch.int32, 2, index)
+    _want(lengths, op, "lengths", torch.int32, 1, index)
+    shape = q.shape
+    tokens = shape[0]
     if lengths.shape[0] != tokens:
         raise ValueError(f"[{op}] lengths must be [tokens].")
+    at_requests = 0
     if requests is not None:
-        _want(requests, op, "requests", torch.int32, 1, device)
+        _want(requests, op, "requests", torch.int32, 1, index)
         if requests.shape[0] != tokens:
             raise ValueError(f"[{op}] requests must be [tokens].")
-    qs = q.stride()
+        at_requests = requests.data_ptr()
+    rows, width = table.shape
     return _QUERIES.pack(
-        q.data_ptr(), tokens, qs[0], qs[1], table.data_ptr(), table.shape[0], table.shape[1],
-        requests.data_ptr() if requests is not None else 0, lengths.data_ptr(), heads,
-        _type(q, op, "q"))
+        q.data_ptr(), tokens, qs[0], qs[1], table.data_ptr(), rows, width, at_requests,
+        lengths.data_ptr(), shape[1], _type(q, op, "q")), shape, index
 
 
-class _On:
-    """Makes a tensor's device current around a call; free when it already is."""
-
-    def __init__(self, device):
-        self.index = device.index
-
-    def __enter__(self):
-        cuda = _torch().cuda
-        self.before = cuda.current_device()
-        if self.before != self.index:
-            cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            _torch().cuda.set_device(self.before)
+def _call(function, args, index, stream):
+    """A C entry with the stream as its last argument, on device `index`."""
+    if stream is None:
+        handle = _current_stream(index)
+    else:
+        handle = stream if isinstance(stream, int) else stream.cuda_stream
+    before = _current_device()
+    if before == index:
+        rc = function(*args, handle)
+    else:
+        with torch.cuda.device(index):
+            rc = function(*args, handle)
+    if rc:
+        _check(rc)
 
 
 def paged_tables(past, fresh, table, free_pages, page_size, num_tokens, *, stream=None):
@@ -142,30 +155,30 @@ def paged_tables(past, fresh, table, free_pages, page_size, num_tokens, *, strea
     """
     op = "mlxvs::paged_tables"
     lib = _load()
-    torch = _torch()
-    if not (_is_torch(past) and past.is_cuda):
+    if not (isinstance(past, torch.Tensor) and past.is_cuda):
         raise ValueError(f"[{op}] past must be a contiguous 1-D CUDA tensor of torch.int32.")
-    device = past.device
-    _want(past, op, "past", torch.int32, 1, device)
-    _want(fresh, op, "fresh", torch.int32, 1, device)
-    _want(table, op, "table", torch.int32, 2, device)
-    _want(free_pages, op, "free_pages", torch.int32, 1, device)
+    index = past.get_device()
+    _want(past, op, "past", torch.int32, 1, index)
+    _want(fresh, op, "fresh", torch.int32, 1, index)
+    _want(table, op, "table", torch.int32, 2, index)
+    _want(free_pages, op, "free_pages", torch.int32, 1, index)
     requests, num_tokens = past.shape[0], int(num_tokens)
-    if fresh.shape[0] != requests or table.shape[0] != requests:
+    rows, width = table.shape
+    if fresh.shape[0] != requests or rows != requests:
         raise ValueError(f"[{op}] past, fresh and table must have one row per request.")
     if num_tokens < 0:
         raise ValueError(f"[{op}] num_tokens must be in [0, 2^31).")
-    with _On(device):
-        slots = torch.empty(num_tokens, dtype=torch.int64, device=device)
-        ints = torch.empty(2 * num_tokens + requests + 3, dtype=torch.int32, device=device)
-        rows, lengths, starts, used = ints.split((num_tokens, num_tokens, requests + 1, 2))
-        at = ints.data_ptr()
-        _check(lib.mlxvs_paged_tables_device(
-            past.data_ptr(), fresh.data_ptr(), requests, int(page_size), free_pages.data_ptr(),
-            free_pages.shape[0], table.data_ptr(), table.shape[1], num_tokens,
-            at + 8 * num_tokens, at, at + 4 * num_tokens, slots.data_ptr(),
-            at + 8 * num_tokens + 4 * (requests + 1), _stream_handle(stream, device)))
-    return PagedTables(starts, rows, lengths, slots, used)
+    slots = past.new_empty(num_tokens, dtype=torch.int64)
+    ints = past.new_empty(2 * num_tokens + requests + 3)
+    at = ints.data_ptr()
+    starts = at + 8 * num_tokens
+    _call(lib.mlxvs_paged_tables_device,
+          (past.data_ptr(), fresh.data_ptr(), requests, int(page_size), free_pages.data_ptr(),
+           free_pages.shape[0], table.data_ptr(), width, num_tokens, starts, at,
+           at + 4 * num_tokens, slots.data_ptr(), starts + 4 * (requests + 1)), index, stream)
+    of, lengths, starts, used = torch.split_with_sizes(
+        ints, (num_tokens, num_tokens, requests + 1, 2))
+    return PagedTables(starts, of, lengths, slots, used)
 
 
 def paged_store(k, v, slots, keys, values, codes=None, scales=None, *, k_scale=1.0, v_scale=1.0,
@@ -177,23 +190,21 @@ def paged_store(k, v, slots, keys, values, codes=None, scales=None, *, k_scale=1
     page that got a row are renewed."""
     op = "mlxvs::paged_store"
     lib = _load()
-    torch = _torch()
-    _rows(k, op, "k", ("tokens", "key heads", "dim"))
-    _rows(v, op, "v", ("tokens", "key heads", "dim"))
-    device = k.device
-    cache = _cache(keys, values, codes, scales, k_scale, v_scale, op, device)
-    if k.shape != v.shape or k.dtype != v.dtype or v.device != device:
+    ks = _rows(k, op, "k", _K_DIMS)
+    vs = _rows(v, op, "v", _K_DIMS)
+    index = k.get_device()
+    cache, shape = _cache(keys, values, codes, scales, k_scale, v_scale, op, index)
+    if k.shape != v.shape or k.dtype is not v.dtype or v.get_device() != index:
         raise ValueError(f"[{op}] k and v must have the same shape, type and device.")
-    if k.shape[1:] != keys.shape[2:]:
+    if k.shape[1:] != shape[2:]:
         raise ValueError(f"[{op}] k and v must have the cache's heads and dimension.")
-    _want(slots, op, "slots", torch.int64, 1, device)
-    if slots.shape[0] != k.shape[0]:
+    tokens = k.shape[0]
+    _want(slots, op, "slots", torch.int64, 1, index)
+    if slots.shape[0] != tokens:
         raise ValueError(f"[{op}] slots must be [tokens].")
-    ks, vs = k.stride(), v.stride()
-    with _On(device):
-        _check(lib.mlxvs_paged_store_device(
-            cache, k.data_ptr(), v.data_ptr(), _type(k, op, "k"), k.shape[0], ks[0], ks[1],
-            vs[0], vs[1], slots.data_ptr(), _stream_handle(stream, device)))
+    _call(lib.mlxvs_paged_store_device,
+          (cache, k.data_ptr(), v.data_ptr(), _type(k, op, "k"), tokens, ks[0], ks[1], vs[0],
+           vs[1], slots.data_ptr()), index, stream)
 
 
 def paged_select(q, codes, scales, table, lengths, page_size, n, *, requests=None, first=1,
@@ -210,21 +221,18 @@ def paged_select(q, codes, scales, table, lengths, page_size, n, *, requests=Non
     """
     op = "mlxvs::paged_select"
     lib = _load()
-    torch = _torch()
     n = int(n)
-    queries = _queries(q, table, lengths, requests, op)
-    if not (_is_torch(codes) and codes.dim() == 4):
+    queries, shape, index = _queries(q, table, lengths, requests, op)
+    if not (isinstance(codes, torch.Tensor) and codes.dim() == 4):
         raise ValueError(f"[{op}] codes must be [pages, key heads, 2, dim] and scales "
                          "[pages, key heads].")
-    pages, heads, _, dim = codes.shape
-    _bounds(codes, scales, op, pages, heads, q.shape[2], q.device)
+    pages, heads = codes.shape[:2]
+    _bounds(codes, scales, op, pages, heads, shape[2], index)
     cache = _CACHE.pack(0, 0, 0, 0, 0, 0, 0, 0, pages, codes.data_ptr(), scales.data_ptr(),
-                        int(page_size), heads, dim, _type(q, op, "q"), 1.0, 1.0)
-    with _On(q.device):
-        out = torch.empty((q.shape[0], heads, max(n, 0)), dtype=torch.int32, device=q.device)
-        _check(lib.mlxvs_paged_select_device(
-            cache, queries, n, int(first), int(last), out.data_ptr(),
-            _stream_handle(stream, q.device)))
+                        int(page_size), heads, shape[2], _type(q, op, "q"), 1.0, 1.0)
+    out = table.new_empty((shape[0], heads, max(n, 0)))
+    _call(lib.mlxvs_paged_select_device,
+          (cache, queries, n, int(first), int(last), out.data_ptr()), index, stream)
     return out
 
 
@@ -241,27 +249,22 @@ def paged_attention(q, keys, values, table, lengths, *, requests=None, pages=Non
     """
     op = "mlxvs::paged_attention"
     lib = _load()
-    torch = _torch()
-    queries = _queries(q, table, lengths, requests, op)
-    device = q.device
-    cache = _cache(keys, values, None, None, k_scale, v_scale, op, device)
-    tokens, q_heads, dim = q.shape
-    if dim != keys.shape[3]:
+    queries, shape, index = _queries(q, table, lengths, requests, op)
+    cache, kv = _cache(keys, values, None, None, k_scale, v_scale, op, index)
+    if shape[2] != kv[3]:
         raise ValueError(f"[{op}] q must have the cache's dimension.")
-    n, selected = 0, None
+    n = at_pages = 0
     if pages is not None:
-        _want(pages, op, "pages", torch.int32, 3, device)
-        n = pages.shape[2]
-        if pages.shape[0] != tokens or pages.shape[1] != keys.shape[2] or n < 1:
+        _want(pages, op, "pages", torch.int32, 3, index)
+        tokens, heads, n = pages.shape
+        if tokens != shape[0] or heads != kv[2] or n < 1:
             raise ValueError(f"[{op}] pages must be [tokens, key heads, n].")
-        selected = pages.data_ptr()
+        at_pages = pages.data_ptr()
     if scale is None:
-        scale = dim ** -0.5
-    with _On(device):
-        out = torch.empty((tokens, q_heads, dim), dtype=q.dtype, device=device)
-        lse = torch.empty((tokens, q_heads), dtype=torch.float32, device=device) \
-            if return_lse else None
-        _check(lib.mlxvs_paged_attention_device(
-            cache, queries, selected, n, scale, out.data_ptr(),
-            lse.data_ptr() if return_lse else None, _stream_handle(stream, device)))
+        scale = shape[2] ** -0.5
+    out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
+    lse = q.new_empty(shape[:2], dtype=torch.float32) if return_lse else None
+    _call(lib.mlxvs_paged_attention_device,
+          (cache, queries, at_pages, n, scale, out.data_ptr(),
+           lse.data_ptr() if return_lse else None), index, stream)
     return (out, lse) if return_lse else out
