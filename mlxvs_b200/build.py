@@ -18,7 +18,8 @@ OBJECTS = os.path.join(HERE, "_build")
 SOURCES = ["engine.cu", "paged.cu", "c_api.cpp", "cpp_api.cu"]
 HEADERS = ["common.cuh", "gemm_topk.cuh", "gemm_topk_q.cuh", "hamming.cuh", "knn_kernels.cuh",
            "select.cuh", "engine.h", "host.h", "paged.h", "paged_common.cuh", "paged_tables.cuh",
-           "paged_store.cuh", "paged_select.cuh", "paged_attention.cuh"]
+           "paged_store.cuh", "paged_select.cuh", "paged_attention.cuh",
+           "paged_prompt.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -27,10 +27,6 @@ namespace mlxvs_b200 {
 
 namespace {
 
-// Bounded waits inside the kernels give up after this long (no legitimate
-// wait comes near it: stages turn over in microseconds).
-constexpr uint64_t WAIT_LIMIT_NS = 2000000000ull;
-
 int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
 // A speculative launch is recorded as PROF_SPECULATIVE until the host knows
@@ -75,28 +71,6 @@ FlagMailbox& flag_mailbox() {
     CK(cudaStreamCreateWithFlags(&b.side, cudaStreamNonBlocking));
   }
   return b;
-}
-
-// cuTensorMapEncodeTiled through the runtime's driver entry point (no link
-// against libcuda).
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
-            cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  });
-  if (!fn) throw std::runtime_error("[mlxvs_b200] cuTensorMapEncodeTiled is unavailable");
-  return fn;
 }
 
 // 2-D fp16 tensor [rows, cols] (cols contiguous), tiles of box_cols x

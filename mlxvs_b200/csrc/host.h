@@ -2,6 +2,7 @@
 // checks, per-device facts, launch profiling and stream-ordered scratch.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -123,5 +124,31 @@ struct Scratch {
     for (void* p : ptrs) cudaFreeAsync(p, s);
   }
 };
+
+// Bounded waits inside the kernels give up after this long (no legitimate
+// wait comes near it: stages turn over in microseconds).
+constexpr uint64_t WAIT_LIMIT_NS = 2000000000ull;
+
+// cuTensorMapEncodeTiled through the runtime's driver entry point (no link
+// against libcuda).
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+inline EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(p);
+  });
+  if (!fn) throw std::runtime_error("[mlxvs_b200] cuTensorMapEncodeTiled is unavailable");
+  return fn;
+}
 
 }  // namespace mlxvs_b200

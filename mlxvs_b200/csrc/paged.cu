@@ -2,10 +2,12 @@
 #include "paged.h"
 
 #include <cmath>
+#include <cstring>
 #include <type_traits>
 
 #include "host.h"
 #include "paged_attention.cuh"
+#include "paged_prompt.cuh"
 #include "paged_select.cuh"
 #include "paged_store.cuh"
 #include "paged_tables.cuh"
@@ -91,10 +93,11 @@ void check_queries(const std::string& op, const mlxvs_paged_cache& c,
           op + "q must be 16-byte aligned, with strides of multiples of 16 bytes.");
 }
 
-// More than 48 KB of dynamic shared memory has to be asked for.
+// More than 48 KB of shared memory, with the kernel's static arrays (at most 16
+// KB here), has to be asked for.
 template <class K>
 void allow_smem(K* kernel, size_t bytes) {
-  if (bytes > 40 * 1024)
+  if (bytes > 32 * 1024)
     CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
 }
 
@@ -125,6 +128,74 @@ void launch_attention(AttentionParams p, DeviceInfo& dev, Scratch& scratch, cuda
   config.attrs = &attribute;
   config.numAttrs = 1;
   CK(cudaLaunchKernelEx(&config, paged_attention_join_kernel<T, DP, NT>, p));
+}
+
+// Keys or values as a 4-D tensor (channel, head, row, page) whose boxes are
+// up to 128 bytes of channels and 64 rows of one head and page.
+template <class C>
+CUtensorMap cache_map(const void* base, const AttentionParams& p, int64_t head_stride,
+                      int64_t row_stride, int64_t page_stride, int box_bytes) {
+  CUtensorMap m;
+  std::memset(&m, 0, sizeof(m));
+  const cuuint64_t size = sizeof(C);
+  const cuuint64_t dims[4] = {(cuuint64_t)p.dim, (cuuint64_t)p.heads, p.page.d,
+                              (cuuint64_t)p.pages};
+  // a dimension of one element may have any stride: one that the map accepts
+  const cuuint64_t strides[3] = {dims[1] > 1 ? head_stride * size : 16,
+                                 dims[2] > 1 ? row_stride * size : 16,
+                                 dims[3] > 1 ? page_stride * size : 16};
+  const cuuint32_t box[4] = {(cuuint32_t)(box_bytes / size), 1, std::min(p.page.d, 64u), 1};
+  const cuuint32_t step[4] = {1, 1, 1, 1};
+  const CUresult r = encode_fn()(
+      &m, size == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 4,
+      const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    throw std::runtime_error("[mlxvs_b200] cuTensorMapEncodeTiled failed: " + std::to_string(r));
+  return m;
+}
+
+// Whether selected pages are walked by tiles of tokens: prompts (more tokens
+// than requests) with enough tiles for the SMs, and a cache that a tensor map
+// can describe.  Pages of under 16 rows would leave most of a stage empty.
+template <class T, class C, int DP>
+bool prompt_tiles(const AttentionParams& p, const DeviceInfo& dev) {
+  using S = PromptShape<T, C, DP>;
+  if (p.selected == nullptr || p.tokens <= p.rows || p.page.d < 16 || p.pages == 0) return false;
+  const int64_t limit = (1LL << 40) / (int64_t)sizeof(C);
+  for (int64_t s : {p.key_page, p.value_page})
+    if (p.pages > 1 && (s == 0 || s >= limit)) return false;
+  for (int64_t s : {p.key_row, p.value_row})
+    if (s == 0 || s >= limit) return false;
+  for (int64_t s : {p.key_head, p.value_head})
+    if (p.heads > 1 && (s == 0 || s >= limit)) return false;
+  const int64_t tile = S::COLUMNS / (p.group > 8 ? 2 : 1);
+  return (p.tokens + tile - 1) / tile * p.heads * ((p.group + 15) / 16) >= dev.sms;
+}
+
+template <class T, class C, int DP>
+void launch_prompt(const AttentionParams& p, DeviceInfo& dev, cudaStream_t s) {
+  using S = PromptShape<T, C, DP>;
+  PromptParams pp;
+  pp.a = p;
+  pp.per_token = p.group > 8 ? 2 : 1;
+  pp.tile = S::COLUMNS / pp.per_token;
+  pp.slots = std::min((int)(p.page.d + 15) / 16 * 16, S::SLOTS);
+  pp.pieces = (int)(p.page.d + S::SLOTS - 1) / S::SLOTS;
+  pp.error = dev.err;
+  pp.limit_ns = WAIT_LIMIT_NS;
+  const CUtensorMap keys =
+      cache_map<C>(p.keys, p, p.key_head, p.key_row, p.key_page, S::BOX);
+  const CUtensorMap values =
+      cache_map<C>(p.values, p, p.value_head, p.value_row, p.value_page, S::BOX);
+  auto* kernel = paged_prompt_kernel<T, C, DP>;
+  allow_smem(kernel, S::SMEM);
+  const dim3 grid((unsigned)((p.tokens + pp.tile - 1) / pp.tile),
+                  p.heads * ((p.group + 15) / 16));
+  ProfScope prof("paged_prompt", s);
+  kernel<<<grid, (S::WARPS + 1) * 32, S::SMEM, s>>>(pp, keys, values);
+  CK(cudaGetLastError());
 }
 
 }  // namespace
@@ -276,7 +347,9 @@ void paged_attention(const mlxvs_paged_cache& c, const mlxvs_paged_queries& q,
           p, dev, scratch, s);
     };
     auto wide = [&](auto dp) {
-      if (p.group <= 8) shaped(dp, std::integral_constant<int, 1>{});
+      if (prompt_tiles<decltype(t), decltype(ct), decltype(dp)::value>(p, dev))
+        launch_prompt<decltype(t), decltype(ct), decltype(dp)::value>(p, dev, s);
+      else if (p.group <= 8) shaped(dp, std::integral_constant<int, 1>{});
       else shaped(dp, std::integral_constant<int, 2>{});
     };
     if (p.dim <= 64) wide(std::integral_constant<int, 64>{});

@@ -76,17 +76,13 @@ def paged_select(q, codes, scales, table, lengths, page_size, n, requests, first
         held = min(-(-max(lengths[t], 0) // page_size), table.shape[1])
         for h in range(heads):
             c = query_codes(q[t, h * group:(h + 1) * group])
-            found = []
-            for b in range(held):
-                p = table[r, b]
-                if not 0 <= p < pages:
-                    continue
-                if b < first or b >= held - last:
-                    score = np.inf
-                else:
-                    score = np.float32((c * codes[p, h]).sum()) * np.float64(scales[p, h])
-                found.append((-score, b))
-            best = sorted(b for _, b in sorted(found)[:n])
+            b = np.arange(held)
+            p = np.asarray(table[r, :held])
+            b, p = b[(p >= 0) & (p < pages)], p[(p >= 0) & (p < pages)]
+            dots = (c * codes[p, h]).sum((1, 2))
+            score = dots.astype(np.float32) * scales[p, h].astype(np.float64)
+            score = np.where((b < first) | (b >= held - last), np.inf, score)
+            best = np.sort(b[np.argsort(-score, kind="stable")[:n]])
             out[t, h, :len(best)] = best
     return out
 

@@ -216,6 +216,15 @@ SELECTED = [
     ([300, 700], [65, 17], 16, 1, 20, 96, 30, "float16", "float8_e4m3fn", "plain"),
     ([4000], [1], 1, 2, 3, 64, 256, "bfloat16", "bfloat16", "plain"),
     ([1500, 1400], [200, 50], 128, 2, 8, 128, 3, "bfloat16", "bfloat16", "plain"),
+    # enough tokens that tiles of them share the pages
+    ([900, 400], [380, 220], 64, 8, 8, 128, 5, "bfloat16", "bfloat16", "plain"),
+    ([777, 5, 333], [300, 5, 290], 24, 8, 6, 80, 7, "float16", "float16", "heads first"),
+    ([1001], [601], 100, 8, 3, 64, 4, "float16", "float8_e4m3fn", "together"),
+    ([500, 300], [200, 90], 16, 4, 12, 256, 9, "bfloat16", "bfloat16", "wide rows"),
+    ([640], [300], 48, 4, 20, 128, 6, "bfloat16", "float8_e4m3fn", "heads first"),
+    ([2500], [560], 1024, 8, 2, 16, 2, "float16", "float8_e4m3fn", "plain"),
+    ([400, 300], [310, 250], 32, 8, 1, 256, 3, "bfloat16", "float8_e4m3fn", "plain"),
+    ([20000], [600], 16, 8, 4, 64, 40, "float16", "float16", "plain"),
 ]
 
 
@@ -252,15 +261,16 @@ def test_select_and_sparse_attention(lengths, fresh, page, heads, group, dim, n,
     assert torch.equal(out, again)
 
 
-def test_sparse_attention_masks():
+@pytest.mark.parametrize("tokens,heads", [(45, 2), (700, 8)])
+def test_sparse_attention_masks(tokens, heads):
     """Lists with gaps, of nothing, beyond the length and the table's holes;
-    tokens of several requests side by side in any order."""
+    tokens of several requests side by side in any order; rows that only the
+    later tokens see and that hold infinities and NaN."""
     rng = np.random.default_rng(8)
-    page, heads, group, dim, n = 16, 2, 8, 128, 6
+    page, group, dim, n = 16, 8, 128, 6
     keys, values = make_cache(rng, 40, page, heads, dim, "bfloat16")
     table = make_table(rng, [200, 150, 90], page, 40, extra=0)
     table[1, 3] = -1
-    tokens = 45
     requests = rng.integers(-1, 4, tokens)
     lengths = rng.integers(0, 210, tokens)
     pages = np.full((tokens, heads, n), -1)
@@ -270,10 +280,25 @@ def test_sparse_attention_masks():
             pages[t, h, rng.permutation(n)[:m]] = rng.permutation(table.shape[1])[:m]
     pages[7] = -1
     q = torch_().from_numpy(rng.standard_normal((tokens, heads * group, dim))).cuda().bfloat16()
-    out, lse = mv.paged_attention(q, keys, values, on_gpu(table), on_gpu(lengths),
-                                  pages=on_gpu(pages), requests=on_gpu(requests), return_lse=True)
+    args = (on_gpu(table), on_gpu(lengths))
+    more = dict(pages=on_gpu(pages), requests=on_gpu(requests), return_lse=True)
+    out, lse = mv.paged_attention(q, keys, values, *args, **more)
     check_attention(out, lse, q, keys, values, table, lengths, requests, dim ** -0.5, "bfloat16",
                     pages)
+    # row 105 of the first request: only tokens that see it may change
+    at = table[0, 105 // page], 105 % page
+    keys[at] = float("nan")
+    values[at] = float("inf")
+    out2, _ = mv.paged_attention(q, keys, values, *args, **more)
+    sees = np.zeros((tokens, heads), bool)
+    for t in range(tokens):
+        for h in range(heads):
+            sees[t, h] = requests[t] == 0 and lengths[t] > 105 and 105 // page in pages[t, h]
+    assert sees.any()
+    sees = on_gpu(sees, "bool")[:, :, None, None]
+    a, b = (x.view(tokens, heads, group, dim) for x in (out, out2))
+    assert torch_().equal(a.masked_fill(sees, 0), b.masked_fill(sees, 0))
+    assert b.masked_select(sees).isnan().all()
 
 
 def test_select_ties_forced_pages_and_odd_queries():
