@@ -56,40 +56,15 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, u
       : "memory");
 }
 
-// mma16816 where `on`, which is the same for the whole warp.
-template <class T>
-__device__ __forceinline__ void mma16816_if(bool on, float (&d)[4], const uint32_t (&a)[4],
-                                            uint32_t b0, uint32_t b1);
-template <>
-__device__ __forceinline__ void mma16816_if<__half>(bool on, float (&d)[4],
-                                                    const uint32_t (&a)[4], uint32_t b0,
-                                                    uint32_t b1) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %10, 0;\n\t"
-      "@p mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7},"
-      " {%8, %9}, {%0, %1, %2, %3};\n\t}\n"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"((int)on));
-}
-template <>
-__device__ __forceinline__ void mma16816_if<__nv_bfloat16>(bool on, float (&d)[4],
-                                                           const uint32_t (&a)[4], uint32_t b0,
-                                                           uint32_t b1) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %10, 0;\n\t"
-      "@p mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3},"
-      " {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n\t}\n"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"((int)on));
-}
-
-// The 16 keys of a stage from slot `first` on, for those of the warp's column
-// groups that see some of them (limit > 0: how many).  One body for all cases,
-// kept short on purpose: the warps are at different pages at any time, and
-// code unrolled over a whole page (or copied for one and two column groups)
-// made them wait for instructions more than for anything else (2.2 ms against
-// 0.6 ms for 5,229 tokens with 16 pages of 64).
-template <class T, class C, int DP, int NT>
+// 16 MT keys of a stage from slot `first` on, for the column groups in WHICH (a
+// bit each); limit: how many of the keys each sees.
+//
+// The bodies are kept short on purpose: the warps are at different pages at
+// any time, and a body unrolled over a whole page made them wait for
+// instructions more than for anything else.  Two independent tiles (of keys,
+// or of column groups) are in flight in each, to cover the latency of the chain
+// products -> weights -> products.
+template <class T, class C, int DP, int NT, int WHICH, int MT>
 __device__ __forceinline__ void prompt_keys(float (&o)[DP / 16][NT][4], float (&m)[NT][2],
                                             float (&l)[NT][2], uint32_t keys, uint32_t values,
                                             uint32_t queries, int first, const int (&limit)[NT],
@@ -104,59 +79,72 @@ __device__ __forceinline__ void prompt_keys(float (&o)[DP / 16][NT][4], float (&
     return (c / PER) * (S::SLOTS * S::BOX) + r * S::BOX + inside * 16;
   };
   // ---- S^T = K Q^T
-  float st[NT][4];
+  float st[MT][NT][4];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) st[nt][0] = st[nt][1] = st[nt][2] = st[nt][3] = 0.0f;
-  const int kr = first + (lane & 15);
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+      st[mt][nt][0] = st[mt][nt][1] = st[mt][nt][2] = st[mt][nt][3] = 0.0f;
 #pragma unroll
   for (int s = 0; s < DP / 16; s += 2) {
     uint32_t q[NT][4];  // operands of steps s and s + 1
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
-      if (limit[nt] > 0)
+      if (WHICH >> nt & 1)
         load_matrices(q[nt], queries + (uint32_t)(nt * 8 + (lane & 7)) * (DP * 2) +
                                  (((2 * s + (lane >> 3)) ^ (lane & 7)) << 4));
-    if (S::EIGHT) {
-      uint32_t a[4];
-      load_matrices(a, keys + chunk_at(kr, s + (lane >> 4)));
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint32_t w[4] = {widen_e4m3(a[2 * u]), widen_e4m3(a[2 * u + 1]),
-                               widen_e4m3(a[2 * u] >> 16), widen_e4m3(a[2 * u + 1] >> 16)};
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          mma16816_if<M>(limit[nt] > 0, st[nt], w, q[nt][2 * u], q[nt][2 * u + 1]);
-      }
-    } else {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
+    for (int mt = 0; mt < MT; ++mt) {
+      const int r = first + mt * 16 + (lane & 15);
+      if (S::EIGHT) {
         uint32_t a[4];
-        load_matrices(a, keys + chunk_at(kr, 2 * (s + u) + (lane >> 4)));
+        load_matrices(a, keys + chunk_at(r, s + (lane >> 4)));
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          mma16816_if<M>(limit[nt] > 0, st[nt], a, q[nt][2 * u], q[nt][2 * u + 1]);
+        for (int u = 0; u < 2; ++u) {
+          const uint32_t w[4] = {widen_e4m3(a[2 * u]), widen_e4m3(a[2 * u + 1]),
+                                 widen_e4m3(a[2 * u] >> 16), widen_e4m3(a[2 * u + 1] >> 16)};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            if (WHICH >> nt & 1) mma16816<M>(st[mt][nt], w, q[nt][2 * u], q[nt][2 * u + 1]);
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          uint32_t a[4];
+          load_matrices(a, keys + chunk_at(r, 2 * (s + u) + (lane >> 4)));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            if (WHICH >> nt & 1) mma16816<M>(st[mt][nt], a, q[nt][2 * u], q[nt][2 * u + 1]);
+        }
       }
     }
   }
-  // ---- weights
-  uint32_t b[NT][2], rest[NT][2];
+  // ---- scores, masked; the maximum is raised where one passes it by 2^8
+  bool raise = false, partial = false;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
-    if (limit[nt] > 0) {
+    if (WHICH >> nt & 1) {
       const float2 f = *reinterpret_cast<const float2*>(&factor[nt][2 * (lane & 3)]);
-      bool raise = false;
+      partial |= limit[nt] < 16 * MT;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float& x = st[nt][i];
-        x *= i & 1 ? f.y : f.x;
-        if ((i >> 1) * 8 + lane / 4 >= limit[nt]) x = -INFINITY;
-        raise |= x > m[nt][i & 1] + 8.0f;
-      }
-      // the maximum is raised where a score passes it by 2^8
-      if (__any_sync(~0u, raise)) {
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float& x = st[mt][nt][i];
+          x *= i & 1 ? f.y : f.x;
+          if (mt * 16 + (i >> 1) * 8 + lane / 4 >= limit[nt]) x = -INFINITY;
+          raise |= x > m[nt][i & 1] + 8.0f;
+        }
+    }
+  if (__any_sync(~0u, raise)) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+      if (WHICH >> nt & 1)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float top = fmaxf(m[nt][i], fmaxf(st[nt][i], st[nt][i + 2]));
+          float top = m[nt][i];
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) top = fmaxf(top, fmaxf(st[mt][nt][i], st[mt][nt][i + 2]));
 #pragma unroll
           for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, w));
           const float keep = m[nt][i] == -INFINITY ? 0.0f : exp2_approx(m[nt][i] - top);
@@ -165,69 +153,84 @@ __device__ __forceinline__ void prompt_keys(float (&o)[DP / 16][NT][4], float (&
 #pragma unroll
           for (int k = 0; k < DP / 16; ++k) o[k][nt][i] *= keep, o[k][nt][i + 2] *= keep;
         }
-      }
+  }
+  // ---- weights
+  uint32_t b[MT][NT][2], rest[MT][NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+    if (WHICH >> nt & 1) {
       const float m0 = m[nt][0] == -INFINITY ? 0.0f : m[nt][0];
       const float m1 = m[nt][1] == -INFINITY ? 0.0f : m[nt][1];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const float w0 = exp2_approx(st[nt][2 * u] - m0);
-        const float w1 = exp2_approx(st[nt][2 * u + 1] - m1);
-        l[nt][0] += w0, l[nt][1] += w1;
-        const uint32_t both = pack2<M>(w0, w1);
-        b[nt][u] = transpose8x8(both);
-        if (TWO_TERMS) {
-          const float2 r = unpack2<M>(both);
-          rest[nt][u] = transpose8x8(pack2<M>(w0 - r.x, w1 - r.y));
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float w0 = exp2_approx(st[mt][nt][2 * u] - m0);
+          const float w1 = exp2_approx(st[mt][nt][2 * u + 1] - m1);
+          l[nt][0] += w0, l[nt][1] += w1;
+          const uint32_t both = pack2<M>(w0, w1);
+          b[mt][nt][u] = transpose8x8(both);
+          if (TWO_TERMS) {
+            const float2 r = unpack2<M>(both);
+            rest[mt][nt][u] = transpose8x8(pack2<M>(w0 - r.x, w1 - r.y));
+          }
+        }
+    }
+  // ---- O^T += V^T P^T
+  auto products = [&](auto masked) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      // Values of keys that a token does not see count as zero, whatever they
+      // hold (a weight of zero times NaN or infinity would not): masks of the
+      // operand's two keys in each half.
+      uint32_t see[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int key = mt * 16 + 8 * u + 2 * (lane & 3);
+          see[nt][u] =
+              (key < limit[nt] ? 0xFFFFu : 0u) | (key + 1 < limit[nt] ? 0xFFFF0000u : 0u);
+        }
+      auto multiply = [&](const uint32_t (&w)[4], int s) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          if (WHICH >> nt & 1) {
+            uint32_t x[4] = {w[0], w[1], w[2], w[3]};
+            if (decltype(masked)::value)
+              x[0] &= see[nt][0], x[1] &= see[nt][0], x[2] &= see[nt][1], x[3] &= see[nt][1];
+            mma16816<M>(o[s][nt], x, b[mt][nt][0], b[mt][nt][1]);
+            if (TWO_TERMS) mma16816<M>(o[s][nt], x, rest[mt][nt][0], rest[mt][nt][1]);
+          }
+      };
+      if (S::EIGHT) {
+        const int r = first + mt * 16 + (lane & 15);
+#pragma unroll
+        for (int s = 0; s < DP / 16; s += 2) {
+          uint32_t a[4];
+          load_matrices_t(a, values + chunk_at(r, s + (lane >> 4)));
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t e0 = __byte_perm(a[2 * u], 0, 0x3120);
+            const uint32_t e1 = __byte_perm(a[2 * u + 1], 0, 0x3120);
+            const uint32_t w[4] = {widen_e4m3(e0), widen_e4m3(e0 >> 16), widen_e4m3(e1),
+                                   widen_e4m3(e1 >> 16)};
+            multiply(w, s + u);
+          }
+        }
+      } else {
+        const int r = first + mt * 16 + (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+          uint32_t a[4];
+          load_matrices_t(a, values + chunk_at(r, 2 * s + ((lane >> 3) & 1)));
+          multiply(a, s);
         }
       }
     }
-  // ---- O^T += V^T P^T.  Values of keys that a token does not see count as
-  // zero, whatever they hold (a weight of zero times NaN or infinity would
-  // not): the masks of the operand's two keys in each half.
-  uint32_t see[NT][2];
-  bool partial = false;
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    partial |= limit[nt] > 0 && limit[nt] < 16;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int key = 8 * u + 2 * (lane & 3);
-      see[nt][u] = (key < limit[nt] ? 0xFFFFu : 0u) | (key + 1 < limit[nt] ? 0xFFFF0000u : 0u);
-    }
-  }
-  auto multiply = [&](const uint32_t (&w)[4], int s) {
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      uint32_t x[4] = {w[0], w[1], w[2], w[3]};
-      if (partial)
-        x[0] &= see[nt][0], x[1] &= see[nt][0], x[2] &= see[nt][1], x[3] &= see[nt][1];
-      mma16816_if<M>(limit[nt] > 0, o[s][nt], x, b[nt][0], b[nt][1]);
-      if (TWO_TERMS) mma16816_if<M>(limit[nt] > 0, o[s][nt], x, rest[nt][0], rest[nt][1]);
-    }
   };
-  if (S::EIGHT) {
-#pragma unroll
-    for (int s = 0; s < DP / 16; s += 2) {
-      uint32_t a[4];
-      load_matrices_t(a, values + chunk_at(kr, s + (lane >> 4)));
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint32_t e0 = __byte_perm(a[2 * u], 0, 0x3120);
-        const uint32_t e1 = __byte_perm(a[2 * u + 1], 0, 0x3120);
-        const uint32_t w[4] = {widen_e4m3(e0), widen_e4m3(e0 >> 16), widen_e4m3(e1),
-                               widen_e4m3(e1 >> 16)};
-        multiply(w, s + u);
-      }
-    }
-  } else {
-    const int vr = first + (lane & 7) + ((lane >> 4) << 3);
-#pragma unroll
-    for (int s = 0; s < DP / 16; ++s) {
-      uint32_t a[4];
-      load_matrices_t(a, values + chunk_at(vr, 2 * s + ((lane >> 3) & 1)));
-      multiply(a, s);
-    }
-  }
+  if (partial) products(std::true_type{});
+  else products(std::false_type{});
 }
 
 template <class T, class C, int DP>
@@ -438,14 +441,33 @@ __global__ void __launch_bounds__((PromptShape<T, C, DP>::WARPS + 1) * 32, 1)
               limit[nt] = mine >> nt & 1 ? min(s_length[warp * NT + nt] - key0, rows) : 0;
               most = max(most, limit[nt]);
             }
-#pragma unroll 1
-            for (int k = 0; k < most; k += 16) {
-              prompt_keys<T, C, DP, NT>(o, m, l, kat, vat,
-                                        q_base + (uint32_t)warp * NT * 8 * DP * 2,
-                                        (e - from) * pp.slots + k, limit,
-                                        &sh_factor[warp * NT]);
+            const int slot = (e - from) * pp.slots;
+            const uint32_t queries = q_base + (uint32_t)warp * NT * 8 * DP * 2;
+            const float(*factor)[8] = &sh_factor[warp * NT];
+            int k = 0;
+            auto step = [&](auto which, auto tiles) {
+              constexpr int MT = decltype(tiles)::value;
+              prompt_keys<T, C, DP, NT, decltype(which)::value, MT>(
+                  o, m, l, kat, vat, queries, slot + k, limit, factor);
+              k += 16 * MT;
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) limit[nt] -= 16;
+              for (int nt = 0; nt < NT; ++nt) limit[nt] -= 16 * MT;
+            };
+            using One = std::integral_constant<int, 1>;
+            using Two = std::integral_constant<int, 2>;
+            using Both = std::integral_constant<int, (1 << NT) - 1>;
+            if (mine == 1) {
+#pragma unroll 1
+              while (k + 32 <= pp.slots && k < most) step(One{}, Two{});
+              if (k < most) step(One{}, One{});
+            } else if (NT == 2 && mine == 2) {
+#pragma unroll 1
+              while (k + 32 <= pp.slots && k < most)
+                step(std::integral_constant<int, NT == 2 ? 2 : 1>{}, Two{});
+              if (k < most) step(std::integral_constant<int, NT == 2 ? 2 : 1>{}, One{});
+            } else if (NT == 2) {
+#pragma unroll 1
+              while (k < most) step(Both{}, One{});
             }
           }
           __syncwarp();
