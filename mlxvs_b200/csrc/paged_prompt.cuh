@@ -22,7 +22,7 @@ namespace mlxvs_b200 {
 template <class T, class C, int DP>
 struct PromptShape {
   static constexpr bool EIGHT = sizeof(C) == 1;
-  static constexpr int WARPS = 15;                 // and one that loads: 4 per SM partition
+  static constexpr int WARPS = 11;                 // and one that loads: 3 per SM partition
   static constexpr int NT = DP == 256 ? 1 : 2;     // column groups (8 heads) of a warp
   static constexpr int COLUMNS = WARPS * NT;       // of a block
   static constexpr int SLOTS = 64;                 // keys of a stage
@@ -30,8 +30,10 @@ struct PromptShape {
   static constexpr int BOXES = DP * (int)sizeof(C) / BOX;  // 128-byte columns of a row
   static constexpr int STAGE = 2 * SLOTS * DP * (int)sizeof(C);
   static constexpr int Q_BYTES = COLUMNS * 8 * DP * 2;
-  static constexpr int STAGES = (131072 / STAGE) < 6 ? (131072 / STAGE) : 6;
   static constexpr int WINDOW = 1024;              // pages marked at a time
+  // what shared memory leaves (227 KB, 4 KB of static arrays and alignment)
+  static constexpr int ROOM = 232448 - 4096 - Q_BYTES - WINDOW * 12;
+  static constexpr int STAGES = ROOM / STAGE < 8 ? ROOM / STAGE : 8;
   static constexpr int SMEM = 1024 + STAGES * STAGE + Q_BYTES + WINDOW * 12;
 };
 
@@ -105,7 +107,8 @@ __device__ __forceinline__ void prompt_keys(float (&o)[DP / 16][NT][4], float (&
                                  widen_e4m3(a[2 * u] >> 16), widen_e4m3(a[2 * u + 1] >> 16)};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
-            if (WHICH >> nt & 1) mma16816<M>(st[mt][nt], w, q[nt][2 * u], q[nt][2 * u + 1]);
+            if (WHICH >> nt & 1)
+              mma16816<M>(st[mt][nt], w, q[nt][2 * u], q[nt][2 * u + 1]);
         }
       } else {
 #pragma unroll
@@ -114,7 +117,8 @@ __device__ __forceinline__ void prompt_keys(float (&o)[DP / 16][NT][4], float (&
           load_matrices(a, keys + chunk_at(r, 2 * (s + u) + (lane >> 4)));
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
-            if (WHICH >> nt & 1) mma16816<M>(st[mt][nt], a, q[nt][2 * u], q[nt][2 * u + 1]);
+            if (WHICH >> nt & 1)
+              mma16816<M>(st[mt][nt], a, q[nt][2 * u], q[nt][2 * u + 1]);
         }
       }
     }
