@@ -471,7 +471,8 @@ __global__ void __launch_bounds__((PromptShape<T, C, DP>::WARPS + 1) * 32, 1)
               if (k < most) step(std::integral_constant<int, NT == 2 ? 2 : 1>{}, One{});
             } else if (NT == 2) {
 #pragma unroll 1
-              while (k < most) step(Both{}, One{});
+              while (k + 32 <= pp.slots && k < most) step(Both{}, Two{});
+              if (k < most) step(Both{}, One{});
             }
           }
           __syncwarp();
