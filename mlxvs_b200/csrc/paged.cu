@@ -297,12 +297,17 @@ void paged_select(const mlxvs_paged_cache& c, const mlxvs_paged_queries& q, int 
   const bool tiles = q.tokens > q.rows && 8 * q.width <= room;
   const int64_t units = (q.tokens + (tiles ? 7 : 0)) / (tiles ? 8 : 1);
   int cluster = 1;
-  while (cluster < 8 && units * c.heads * cluster < dev.sms && cluster * 128 < q.width)
+  while (cluster < 8 && units * c.heads * cluster < 2 * dev.sms && cluster * 128 < q.width)
     cluster *= 2;
   ProfScope prof("paged_select", s);
   dispatch_types(q.type, q.type, [&](auto t, auto) {
     using T = decltype(t);
-    auto* kernel = tiles ? paged_select_kernel<T, 8> : paged_select_kernel<T, 1>;
+    auto* kernel = p.dim <= 64    ? tiles ? paged_select_kernel<T, 8, 2>
+                                          : paged_select_kernel<T, 1, 2>
+                   : p.dim <= 128 ? tiles ? paged_select_kernel<T, 8, 4>
+                                          : paged_select_kernel<T, 1, 4>
+                   : tiles        ? paged_select_kernel<T, 8, 8>
+                                  : paged_select_kernel<T, 1, 8>;
     const size_t smem = (size_t)(tiles ? 8 : 1) * q.width * 4;
     allow_smem(kernel, smem);
     cudaLaunchConfig_t config = {};
