@@ -156,11 +156,16 @@ struct AttentionShape {
   static constexpr int PART = HEADS * (DP + 2);  // floats of a partial result
 };
 
-// The row (token, key head, chunk of query heads) of a tile of the sequence.
+// A row's end (joining the warps, writing, fetching queries) takes as long as
+// about this many tiles, so it counts as such in the cut of the work: without
+// it the blocks that got many short rows were the last to end by far.
+constexpr int ROW_COST = 2;
+
+// The row (token, key head, chunk of query heads) of a place in the sequence.
 struct AttentionRow {
   int64_t t;       // token
   int h, chunk;    // key head, chunk of query heads
-  int64_t start;   // the row's first tile
+  int64_t start;   // the place of the row's first tile, behind its cost
   int tiles;
 };
 
@@ -210,24 +215,25 @@ __global__ void __launch_bounds__(AttentionShape<T, C, DP, NT>::WARPS * 32,
     return max(1, (length_of(t) + S::KEYS - 1) / S::KEYS);
   };
 
-  // ---- this block's range of tiles, and the row it begins in
+  // ---- this block's range of places, and the row it begins in
   int64_t total;
   int64_t x, x1, per;
   AttentionRow row;
   if (SPARSE) {
     row.tiles = tiles_of(0);
-    total = p.tokens * per_token * row.tiles;
+    const int places = row.tiles + ROW_COST;
+    total = p.tokens * per_token * places;
     per = max((int64_t)1, (total + gridDim.x - 1) / gridDim.x);
     x = blockIdx.x * per, x1 = min(x + per, total);
-    const int64_t index = x / row.tiles;
+    const int64_t index = x / places;
     row.t = index / per_token;
-    row.start = index * row.tiles;
+    row.start = index * places + ROW_COST;
     row.h = (int)(index % per_token) / chunks, row.chunk = (int)(index % per_token) % chunks;
   } else {
     const int64_t each = (p.tokens + THREADS - 1) / THREADS;
     const int64_t ta = min(tid * each, p.tokens), tb = min(ta + each, p.tokens);
     int64_t mine = 0;
-    for (int64_t t = ta; t < tb; ++t) mine += tiles_of(t);
+    for (int64_t t = ta; t < tb; ++t) mine += tiles_of(t) + ROW_COST;
     int64_t sum = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -249,7 +255,7 @@ __global__ void __launch_bounds__(AttentionShape<T, C, DP, NT>::WARPS * 32,
     int64_t at = before * per_token;
     if (x >= at && x < at + mine * per_token)
       for (int64_t t = ta; t < tb; ++t) {
-        const int64_t next = at + (int64_t)tiles_of(t) * per_token;
+        const int64_t next = at + (int64_t)(tiles_of(t) + ROW_COST) * per_token;
         if (x < next) {
           sh_found[0] = t, sh_found[1] = at;
           break;
@@ -260,22 +266,24 @@ __global__ void __launch_bounds__(AttentionShape<T, C, DP, NT>::WARPS * 32,
     if (x < x1) {
       row.t = sh_found[0];
       row.tiles = tiles_of(row.t);
-      const int index = (int)((x - sh_found[1]) / row.tiles);
-      row.start = sh_found[1] + (int64_t)index * row.tiles;
+      const int places = row.tiles + ROW_COST;
+      const int index = (int)((x - sh_found[1]) / places);
+      row.start = sh_found[1] + (int64_t)index * places + ROW_COST;
       row.h = index / chunks, row.chunk = index % chunks;
     }
   }
-  if (x >= x1) {
-    if (tid == 0) p.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
-    return;
-  }
+  // the block's first tile, and how many places are left from there: a range
+  // that ends within a row's cost leaves the row to the next block
+  const bool cut = x < x1 && x > row.start;
   if (tid == 0) {
-    // the row that this block's start cuts, listed by the first block that cuts it
-    const bool first = row.start < x && row.start >= x - per;
-    const int64_t last = (row.start + row.tiles - 1) / per;
+    // a row that this block's start cuts, listed by the first block that cuts it
+    const bool first = cut && row.start >= x - per;
+    const int64_t last = first ? (row.start + row.tiles - 1) / per : 0;
     p.cut[blockIdx.x] =
         first ? make_int4((int)row.t, row.h, row.chunk, (int)last) : make_int4(-1, 0, 0, 0);
   }
+  x = max(x, row.start);
+  if (x >= x1) return;
 
   const uint32_t my_ring = smem_address(ring) + warp * S::STAGES * S::STEP;
   // columns past dim are never copied: zero for good
@@ -293,102 +301,130 @@ __global__ void __launch_bounds__(AttentionShape<T, C, DP, NT>::WARPS * 32,
     return r * S::PITCH + s * 16;
   };
 
-  while (x < x1) {
-    // ------------------------------------------------ one row's piece
-    const int64_t t = row.t;
-    const int h = row.h;
-    const int tile0 = (int)(x - row.start);
-    const int tile1 = (int)(min(x1, row.start + row.tiles) - row.start);
+  // ---- the loading side runs STAGES - 1 tiles ahead of the products, across
+  // the ends of rows: while one row's results are written, the next one's
+  // first tiles are on their way
+  struct {
+    int64_t t;
+    int h, chunk, tile, tiles, length;
+    const int32_t* table;
+  } ahead;
+  auto enter = [&](int64_t t) {  // the loading side's token
     const int64_t request = p.requests ? p.requests[t] : t;
-    const int length = length_of(t);
-    const int32_t* table = p.table + request * p.width;
-    const int32_t* selected =
-        SPARSE ? p.selected + (t * p.heads + h) * p.n : nullptr;
-    const int head0 = h * p.group + row.chunk * S::HEADS;  // first query head
-    const int heads = min(S::HEADS, p.group - row.chunk * S::HEADS);
-    const C* keys = static_cast<const C*>(p.keys) + h * p.key_head;
-    const C* values = static_cast<const C*>(p.values) + h * p.value_head;
-
-    // where this lane's key of a tile lies: page (-1: none) and row in it
-    auto locate = [&](int tile, int& page, int& in) {
-      page = -1, in = 0;
-      if (lane >= KT || tile >= tile1) return;
-      const int64_t j = (int64_t)tile * S::KEYS + warp * KT + lane;
-      int b;
+    ahead.t = t;
+    ahead.length = length_of(t);
+    ahead.table = p.table + request * p.width;
+    if (!SPARSE) ahead.tiles = max(1, (ahead.length + S::KEYS - 1) / S::KEYS);
+  };
+  ahead.h = row.h, ahead.chunk = row.chunk, ahead.tile = (int)(x - row.start);
+  ahead.tiles = row.tiles;
+  enter(row.t);
+  // where this lane's key of the next tile lies: page (-1: none), row in it and
+  // key head
+  int page, in, page_head;
+  bool located;  // there is a next tile
+  int64_t ahead_x = x;
+  auto locate = [&] {
+    page = -1, in = 0, page_head = ahead.h;
+    located = ahead_x < x1;
+    if (!located) return;
+    const int64_t j = (int64_t)ahead.tile * S::KEYS + warp * KT + lane;
+    if (lane < KT) {
       if (SPARSE) {
-        if (j >= (int64_t)p.n * P) return;
-        const int pos = (int)p.page.div((uint32_t)j);
-        in = (int)j - pos * P;
-        b = selected[pos];
-        if (b < 0 || b >= p.width || (int64_t)b * P + in >= length) return;
-      } else {
-        if (j >= length) return;
-        b = (int)p.page.div((uint32_t)j);
+        if (j < (int64_t)p.n * P) {
+          const int pos = (int)p.page.div((uint32_t)j);
+          in = (int)j - pos * P;
+          const int b = p.selected[(ahead.t * p.heads + ahead.h) * p.n + pos];
+          if (b >= 0 && b < p.width && (int64_t)b * P + in < ahead.length) page = ahead.table[b];
+        }
+      } else if (j < ahead.length) {
+        const int b = (int)p.page.div((uint32_t)j);
         in = (int)j - b * P;
+        page = ahead.table[b];
       }
-      page = table[b];
-    };
-    auto load = [&](int stage, int page, int in) {
-      if (page >= p.pages) page = -1;
-      const uint32_t valid = __ballot_sync(~0u, page >= 0);
-      if (lane == 0) sh_valid[warp][stage] = valid;
-      const uint32_t at = my_ring + stage * S::STEP;
-      constexpr int LANES = CH < 8 ? CH : 8;  // lanes of a row
-      constexpr int ROWS = 32 / LANES;
-#pragma unroll
-      for (int g = 0; g < KT / ROWS; ++g) {
-        const int r = g * ROWS + lane / LANES;
-        const int64_t pg = __shfl_sync(~0u, page, r);
-        const int64_t i = __shfl_sync(~0u, in, r);
-        const C* k = keys + pg * p.key_page + i * p.key_row;
-        const C* v = values + pg * p.value_page + i * p.value_row;
-#pragma unroll
-        for (int cc = 0; cc < CH; cc += LANES) {
-          const int c = cc + lane % LANES;
-          if (c * (16 / (int)sizeof(C)) < p.dim) {
-            const uint32_t to = at + chunk_at(r, c);
-            copy16(to, pg >= 0 ? k + c * (16 / sizeof(C)) : keys, pg >= 0);
-            copy16(to + KT * S::PITCH, pg >= 0 ? v + c * (16 / sizeof(C)) : values, pg >= 0);
-          }
+    }
+    ++ahead_x;
+    if (++ahead.tile == ahead.tiles) {
+      ahead.tile = 0;
+      ahead_x += ROW_COST;
+      if (++ahead.chunk == chunks) {
+        ahead.chunk = 0;
+        if (++ahead.h == p.heads) {
+          ahead.h = 0;
+          if (ahead.t + 1 < p.tokens) enter(ahead.t + 1);
         }
       }
-    };
-
-    int page, in;
-    locate(tile0, page, in);
-#pragma unroll
-    for (int s = 0; s < S::STAGES - 1; ++s) {
-      if (tile0 + s < tile1) load(s, page, in);
-      copy_commit();
-      locate(tile0 + s + 1, page, in);
     }
+  };
+  auto load = [&](int stage) {
+    if (page >= p.pages) page = -1;
+    const uint32_t valid = __ballot_sync(~0u, page >= 0);
+    if (lane == 0) sh_valid[warp][stage] = valid;
+    const uint32_t at = my_ring + stage * S::STEP;
+    const C* keys = static_cast<const C*>(p.keys) + page_head * p.key_head;
+    const C* values = static_cast<const C*>(p.values) + page_head * p.value_head;
+    constexpr int LANES = CH < 8 ? CH : 8;  // lanes of a row
+    constexpr int ROWS = 32 / LANES;
+#pragma unroll
+    for (int g = 0; g < KT / ROWS; ++g) {
+      const int r = g * ROWS + lane / LANES;
+      const int64_t pg = __shfl_sync(~0u, page, r);
+      const int64_t i = __shfl_sync(~0u, in, r);
+      const C* k = keys + pg * p.key_page + i * p.key_row;
+      const C* v = values + pg * p.value_page + i * p.value_row;
+#pragma unroll
+      for (int cc = 0; cc < CH; cc += LANES) {
+        const int c = cc + lane % LANES;
+        if (c * (16 / (int)sizeof(C)) < p.dim) {
+          const uint32_t to = at + chunk_at(r, c);
+          copy16(to, pg >= 0 ? k + c * (16 / sizeof(C)) : keys, pg >= 0);
+          copy16(to + KT * S::PITCH, pg >= 0 ? v + c * (16 / sizeof(C)) : values, pg >= 0);
+        }
+      }
+    }
+  };
+  locate();
+#pragma unroll
+  for (int s = 0; s < S::STAGES - 1; ++s) {
+    if (located) load(s);
+    copy_commit();
+    locate();
+  }
 
-    // ---- queries: B operands, head n = lane / 4 of each eight
-    uint32_t qf[DP / 16][NT][2];
-    float factor[NT][2];  // of the scores of heads 2 (lane % 4) + {0, 1}
-    const T* q = static_cast<const T*>(p.q) + t * p.q_token + head0 * p.q_head;
+  // ---- queries: B operands, head n = lane / 4 of each eight
+  uint32_t qf[DP / 16][NT][2];
+  float factor[NT][2];  // of the scores of heads 2 (lane % 4) + {0, 1}
+  auto fetch_queries = [&] {
+    const int head0 = row.h * p.group + row.chunk * S::HEADS;
+    const int heads = min(S::HEADS, p.group - row.chunk * S::HEADS);
+    const T* q = static_cast<const T*>(p.q) + row.t * p.q_token + (int64_t)head0 * p.q_head;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int n = nt * 8 + lane / 4;
       const T* qn = q + (int64_t)min(n, heads - 1) * p.q_head;
-      float top = 0.0f;
 #pragma unroll
       for (int s = 0; s < DP / 16; ++s) {
         const int d0 = s * 16 + (S::EIGHT ? 4 : 2) * (lane % 4), d1 = d0 + (S::EIGHT ? 2 : 8);
         const bool live = n < heads;
         qf[s][nt][0] = live && d0 < p.dim ? *reinterpret_cast<const uint32_t*>(qn + d0) : 0u;
         qf[s][nt][1] = live && d1 < p.dim ? *reinterpret_cast<const uint32_t*>(qn + d1) : 0u;
-        if (S::EIGHT) {
+      }
+    }
+  };
+  auto scale_queries = [&] {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      factor[nt][0] = factor[nt][1] = p.scale;
+      if (S::EIGHT) {
+        // the largest magnitude to [64, 128): exact in float16 down to 2^-21 of it
+        float top = 0.0f;
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const float2 v = unpack2<T>(qf[s][nt][i]);
             top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
           }
-        }
-      }
-      factor[nt][0] = factor[nt][1] = p.scale;
-      if (S::EIGHT) {
-        // the largest magnitude to [64, 128): exact in float16 down to 2^-21 of it
         top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
         top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
         const int e = code_exponent(top);
@@ -405,7 +441,15 @@ __global__ void __launch_bounds__(AttentionShape<T, C, DP, NT>::WARPS * 32,
           factor[nt][i] = __shfl_sync(~0u, back, (2 * (lane % 4) + i) * 4);
       }
     }
+  };
+  fetch_queries();
 
+  int stage = 0;
+  while (x < x1) {
+    // ------------------------------------------------ one row's piece
+    const int tile0 = (int)(x - row.start);
+    const int tile1 = (int)min((int64_t)row.tiles, x1 - row.start);
+    scale_queries();
     float o[DP / 16][NT][4], m[NT][2], l[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -415,16 +459,15 @@ __global__ void __launch_bounds__(AttentionShape<T, C, DP, NT>::WARPS * 32,
         o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.0f;
     }
 
-    int stage = 0;
     for (int tile = tile0; tile < tile1; ++tile) {
       copy_wait<S::STAGES - 2>();
       __syncwarp();
       {
         int to = stage + S::STAGES - 1;
         if (to >= S::STAGES) to -= S::STAGES;
-        if (tile + S::STAGES - 1 < tile1) load(to, page, in);
+        if (located) load(to);
         copy_commit();
-        locate(tile + S::STAGES, page, in);
+        locate();
       }
       const uint32_t valid = sh_valid[warp][stage];
       const uint32_t kat = my_ring + stage * S::STEP, vat = kat + KT * S::PITCH;
@@ -554,7 +597,17 @@ __global__ void __launch_bounds__(AttentionShape<T, C, DP, NT>::WARPS * 32,
         }
       }
     }
-    copy_wait<0>();
+    // ---- on to the next row, whose queries are fetched meanwhile
+    const AttentionRow ended = row;
+    row.start += row.tiles + ROW_COST;
+    x = row.start;
+    if (x < x1) {
+      if (++row.chunk == chunks) {
+        row.chunk = 0;
+        if (++row.h == p.heads) row.h = 0, row.t += 1, row.tiles = tiles_of(row.t);
+      }
+      fetch_queries();
+    }
 
     // ---- join the warps in their order
 #pragma unroll
@@ -599,7 +652,9 @@ __global__ void __launch_bounds__(AttentionShape<T, C, DP, NT>::WARPS * 32,
       __syncthreads();
     }
     // ---- write the row, or its part
-    const bool whole = tile0 == 0 && tile1 == row.tiles;
+    const bool whole = tile0 == 0 && tile1 == ended.tiles;
+    const int head0 = ended.h * p.group + ended.chunk * S::HEADS;  // first query head
+    const int heads = min(S::HEADS, p.group - ended.chunk * S::HEADS);
     float* part = p.part + ((int64_t)blockIdx.x * 2 + (tile0 == 0)) * S::PART;
     for (int n = warp; n < heads; n += S::WARPS) {
       float top = -INFINITY, sum = 0.0f;
@@ -609,7 +664,7 @@ __global__ void __launch_bounds__(AttentionShape<T, C, DP, NT>::WARPS * 32,
       for (int w = 0; w < S::WARPS; ++w)
         sum += sh_m[w][n] == -INFINITY ? sh_l[w][n] : sh_l[w][n] * exp2_approx(sh_m[w][n] - top);
       if (whole) {
-        const int64_t hq = t * p.heads * p.group + head0 + n;
+        const int64_t hq = ended.t * p.heads * p.group + head0 + n;
         T* out = static_cast<T*>(p.out) + hq * p.dim;
         const float by = sum != 0.0f ? p.v_scale / sum : 0.0f;
         for (int d = 2 * lane; d < p.dim; d += 64) {
@@ -624,17 +679,8 @@ __global__ void __launch_bounds__(AttentionShape<T, C, DP, NT>::WARPS * 32,
       }
     }
     __syncthreads();
-
-    // ---- the next row
-    x += tile1 - tile0;
-    if (x < x1) {
-      row.start += row.tiles;
-      if (++row.chunk == chunks) {
-        row.chunk = 0;
-        if (++row.h == p.heads) row.h = 0, row.t += 1, row.tiles = tiles_of(row.t);
-      }
-    }
   }
+  copy_wait<0>();
 }
 
 // Joins the parts of a cut row, one block per cut and query head: parts in the
