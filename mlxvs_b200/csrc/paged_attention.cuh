@@ -42,8 +42,13 @@ __device__ __forceinline__ uint32_t smem_address(const void* p) {
   return (uint32_t)__cvta_generic_to_shared(p);
 }
 
-// 16 bytes to shared memory past L1; zeros where !valid (src is not read).
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool valid) {
+// 16 bytes to shared memory, past L1.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src)
+               : "memory");
+}
+// Zeros where !valid (src is not read then).
+__device__ __forceinline__ void copy16_or_zero(uint32_t dst, const void* src, bool valid) {
   asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
                "r"(valid ? 16 : 0)
                : "memory");
@@ -147,8 +152,12 @@ struct AttentionShape {
   static constexpr int KT = PITCH <= 128 ? 32 : 16;  // keys of a warp's step
   static constexpr int STEP = 2 * KT * PITCH;        // bytes of a warp's step
   static constexpr int WARPS = 4;
-  static constexpr int BLOCKS = STEP > 8192 ? 1 : 2;  // per SM
-  static constexpr int STAGES = STEP > 8192 ? 3 : STEP > 4096 ? 3 : 6;
+  // Blocks per SM, as registers allow, and the ring that shared memory leaves
+  // each: three blocks with rings of two steps against two with three took
+  // 166 for 175 us on long 8-bit caches, and 20 for 23 us on short lists of pages
+  // (the products' latency counts there), the same on others.
+  static constexpr int BLOCKS = STEP > 8192 ? 1 : NT == 1 && DP <= 128 ? 3 : 2;
+  static constexpr int STAGES = STEP > 8192 ? 3 : (BLOCKS == 3 ? 2 : 3) * (8192 / STEP);
   static constexpr int KEYS = WARPS * KT;  // keys of a tile
   static constexpr int HEADS = 8 * NT;
   static constexpr int RING = WARPS * STAGES * STEP;
@@ -319,29 +328,27 @@ __global__ void __launch_bounds__(AttentionShape<T, C, DP, NT>::WARPS * 32,
   ahead.h = row.h, ahead.chunk = row.chunk, ahead.tile = (int)(x - row.start);
   ahead.tiles = row.tiles;
   enter(row.t);
-  // where this lane's key of the next tile lies: page (-1: none), row in it and
-  // key head
-  int page, in, page_head;
+  // where this lane's key of the next tile lies: its page (-1: none) and the
+  // offsets of its row in it, with the key head's
+  int page;
+  int64_t key_at, value_at;
   bool located;  // there is a next tile
   int64_t ahead_x = x;
   auto locate = [&] {
-    page = -1, in = 0, page_head = ahead.h;
+    page = -1;
     located = ahead_x < x1;
     if (!located) return;
     const int64_t j = (int64_t)ahead.tile * S::KEYS + warp * KT + lane;
-    if (lane < KT) {
+    if (lane < KT && j < (SPARSE ? (int64_t)p.n * P : (int64_t)ahead.length)) {
+      const int pos = (int)p.page.div((uint32_t)j), in = (int)j - pos * P;
+      int b = pos;
       if (SPARSE) {
-        if (j < (int64_t)p.n * P) {
-          const int pos = (int)p.page.div((uint32_t)j);
-          in = (int)j - pos * P;
-          const int b = p.selected[(ahead.t * p.heads + ahead.h) * p.n + pos];
-          if (b >= 0 && b < p.width && (int64_t)b * P + in < ahead.length) page = ahead.table[b];
-        }
-      } else if (j < ahead.length) {
-        const int b = (int)p.page.div((uint32_t)j);
-        in = (int)j - b * P;
-        page = ahead.table[b];
+        b = p.selected[(ahead.t * p.heads + ahead.h) * p.n + pos];
+        if (b >= p.width || (int64_t)b * P + in >= ahead.length) b = -1;
       }
+      if (b >= 0) page = ahead.table[b];
+      key_at = in * p.key_row + ahead.h * p.key_head;
+      value_at = in * p.value_row + ahead.h * p.value_head;
     }
     ++ahead_x;
     if (++ahead.tile == ahead.tiles) {
@@ -360,26 +367,44 @@ __global__ void __launch_bounds__(AttentionShape<T, C, DP, NT>::WARPS * 32,
     if (page >= p.pages) page = -1;
     const uint32_t valid = __ballot_sync(~0u, page >= 0);
     if (lane == 0) sh_valid[warp][stage] = valid;
-    const uint32_t at = my_ring + stage * S::STEP;
-    const C* keys = static_cast<const C*>(p.keys) + page_head * p.key_head;
-    const C* values = static_cast<const C*>(p.values) + page_head * p.value_head;
+    // offsets in bytes from the first key and value
+    const int64_t koff = (page * p.key_page + key_at) * (int64_t)sizeof(C);
+    const int64_t voff = (page * p.value_page + value_at) * (int64_t)sizeof(C);
     constexpr int LANES = CH < 8 ? CH : 8;  // lanes of a row
     constexpr int ROWS = 32 / LANES;
+    const int c0 = lane % LANES, r0 = lane / LANES;
+    const uint8_t* keys = static_cast<const uint8_t*>(p.keys) + c0 * 16;
+    const uint8_t* values = static_cast<const uint8_t*>(p.values) + c0 * 16;
+    const uint32_t at = my_ring + stage * S::STEP;
+    const int bytes = p.dim * (int)sizeof(C) - c0 * 16;  // of a row, from this lane's chunk
+    if (valid == (KT == 32 ? ~0u : (1u << KT) - 1)) {
 #pragma unroll
-    for (int g = 0; g < KT / ROWS; ++g) {
-      const int r = g * ROWS + lane / LANES;
-      const int64_t pg = __shfl_sync(~0u, page, r);
-      const int64_t i = __shfl_sync(~0u, in, r);
-      const C* k = keys + pg * p.key_page + i * p.key_row;
-      const C* v = values + pg * p.value_page + i * p.value_row;
+      for (int g = 0; g < KT / ROWS; ++g) {
+        const int r = g * ROWS + r0;
+        const uint8_t* k = keys + __shfl_sync(~0u, koff, r);
+        const uint8_t* v = values + __shfl_sync(~0u, voff, r);
 #pragma unroll
-      for (int cc = 0; cc < CH; cc += LANES) {
-        const int c = cc + lane % LANES;
-        if (c * (16 / (int)sizeof(C)) < p.dim) {
-          const uint32_t to = at + chunk_at(r, c);
-          copy16(to, pg >= 0 ? k + c * (16 / sizeof(C)) : keys, pg >= 0);
-          copy16(to + KT * S::PITCH, pg >= 0 ? v + c * (16 / sizeof(C)) : values, pg >= 0);
-        }
+        for (int cc = 0; cc < CH; cc += LANES)
+          if (cc * 16 < bytes) {
+            const uint32_t to = at + chunk_at(r, cc + c0);
+            copy16(to, k + cc * 16);
+            copy16(to + KT * S::PITCH, v + cc * 16);
+          }
+      }
+    } else {
+      // rows that are not there become zeros
+#pragma unroll
+      for (int g = 0; g < KT / ROWS; ++g) {
+        const int r = g * ROWS + r0;
+        const bool there = valid >> r & 1;
+        const int64_t ko = __shfl_sync(~0u, koff, r), vo = __shfl_sync(~0u, voff, r);
+#pragma unroll
+        for (int cc = 0; cc < CH; cc += LANES)
+          if (cc * 16 < bytes) {
+            const uint32_t to = at + chunk_at(r, cc + c0);
+            copy16_or_zero(to, there ? keys + ko + cc * 16 : keys, there);
+            copy16_or_zero(to + KT * S::PITCH, there ? values + vo + cc * 16 : values, there);
+          }
       }
     }
   };
