@@ -226,7 +226,11 @@ void paged_tables(const int32_t* past, const int32_t* fresh, int64_t requests, i
   const unsigned blocks =
       (unsigned)std::max<int64_t>(1, (num_tokens + TABLES_TOKENS - 1) / TABLES_TOKENS);
   ProfScope prof("paged_tables", s);
-  paged_tables_kernel<<<blocks, TABLES_THREADS, 0, s>>>(p);
+  // one pass over up to 256 requests, or 1024 (a request a thread is quicker)
+  if (requests <= TABLES_THREADS)
+    paged_tables_kernel<1><<<blocks, TABLES_THREADS, 0, s>>>(p);
+  else
+    paged_tables_kernel<4><<<blocks, TABLES_THREADS, 0, s>>>(p);
   CK(cudaGetLastError());
 }
 

@@ -12,6 +12,7 @@
 
 #include <type_traits>
 
+#include "paged_attention.cuh"
 #include "paged_common.cuh"
 
 namespace mlxvs_b200 {
@@ -36,6 +37,57 @@ constexpr int STORE_WARPS = 8;
 template <class T>
 struct alignas(sizeof(T) * 8) Eight {
   T x[8];
+};
+
+// Eight values times `by`, rounded to C.
+template <class T, class C>
+__device__ __forceinline__ Eight<C> rounded(const Eight<T>& x, float by) {
+  Eight<C> y;
+  if (std::is_same<T, C>::value && by == 1.0f) return *reinterpret_cast<const Eight<C>*>(&x);
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&x);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = unpack2<T>(w[i]);
+    if (sizeof(C) == 1) {
+      reinterpret_cast<__nv_fp8x2_storage_t*>(&y)[i] = __nv_cvt_float2_to_fp8x2(
+          make_float2(v.x * by, v.y * by), __NV_SATFINITE, __NV_E4M3);
+    } else {
+      reinterpret_cast<uint32_t*>(&y)[i] = pack2<T>(v.x * by, v.y * by);
+    }
+  }
+  return y;
+}
+
+// Running minima and maxima of eight channels in pairs of 16-bit values.  NaN is
+// passed over; scaling by a positive number and rounding keep the order, so
+// the bounds of what is stored are the stored bounds of the input.
+template <class T>
+struct Range;
+template <>
+struct Range<__half> {
+  __half2 lo[4], hi[4];
+  __device__ __forceinline__ Range() {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      lo[i] = __float2half2_rn(INFINITY), hi[i] = __float2half2_rn(-INFINITY);
+  }
+  __device__ __forceinline__ void take(int i, uint32_t w) {
+    const __half2 x = *reinterpret_cast<const __half2*>(&w);
+    lo[i] = __hmin2(lo[i], x), hi[i] = __hmax2(hi[i], x);
+  }
+};
+template <>
+struct Range<__nv_bfloat16> {
+  __nv_bfloat162 lo[4], hi[4];
+  __device__ __forceinline__ Range() {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      lo[i] = __float2bfloat162_rn(INFINITY), hi[i] = __float2bfloat162_rn(-INFINITY);
+  }
+  __device__ __forceinline__ void take(int i, uint32_t w) {
+    const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162*>(&w);
+    lo[i] = __hmin2(lo[i], x), hi[i] = __hmax2(hi[i], x);
+  }
 };
 
 // One warp per key head and chunk of up to 32 tokens, LANES lanes per row (8
@@ -74,15 +126,6 @@ __global__ void __launch_bounds__(STORE_WARPS * 32)
       last = !(row + 1 < P && t0 + lane + 1 < p.tokens && p.slots[t0 + lane + 1] == slot + 1);
     }
   }
-  auto rounded = [](const Eight<T>& x, float by) {
-    Eight<C> y;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      y.x[i] = std::is_same<T, C>::value && by == 1.0f
-                   ? *reinterpret_cast<const C*>(&x.x[i])
-                   : from_float<C>(to_float(x.x[i]) * by);
-    return y;
-  };
   constexpr int UNROLL = 4;
   for (int i0 = 0; i0 < count; i0 += ROWS * UNROLL) {
     Eight<T> kx[UNROLL], vx[UNROLL];
@@ -102,9 +145,9 @@ __global__ void __launch_bounds__(STORE_WARPS * 32)
     for (int u = 0; u < UNROLL; ++u)
       if (pg[u] >= 0) {
         *reinterpret_cast<Eight<C>*>(keys + pg[u] * p.key_page + r[u] * p.key_row) =
-            rounded(kx[u], p.k_inverse);
+            rounded<T, C>(kx[u], p.k_inverse);
         *reinterpret_cast<Eight<C>*>(values + pg[u] * p.value_page + r[u] * p.value_row) =
-            rounded(vx[u], p.v_inverse);
+            rounded<T, C>(vx[u], p.v_inverse);
       }
   }
   if (p.codes == nullptr) return;
@@ -124,25 +167,49 @@ __global__ void __launch_bounds__(STORE_WARPS * 32)
       begin -= run;
       if (run < 32) break;
     }
-    float lo[8], hi[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) lo[i] = INFINITY, hi[i] = -INFINITY;
-    auto take = [&](const Eight<C>& x) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float y = to_float(x.x[i]);  // fminf and fmaxf pass over NaN
-        lo[i] = fminf(lo[i], y), hi[i] = fmaxf(hi[i], y);
-      }
-    };
+    // old rows as they are stored (e4m3 as the float16 it is exactly), new ones
+    // as they came
+    using Old = typename std::conditional<sizeof(C) == 1, __half, T>::type;
+    Range<Old> old_range;
+    Range<T> new_range;
     if (mine) {
       const C* old = keys + pg * p.key_page;
 #pragma unroll 8
-      for (int r = sub; r < begin; r += ROWS)
-        take(*reinterpret_cast<const Eight<C>*>(old + r * p.key_row));
-#pragma unroll 4
-      for (int r = begin + sub; r <= re; r += ROWS)
-        take(rounded(*reinterpret_cast<const Eight<T>*>(k + (te - (re - r)) * p.k_token),
-                     p.k_inverse));
+      for (int r = sub; r < begin; r += ROWS) {
+        const Eight<C> x = *reinterpret_cast<const Eight<C>*>(old + r * p.key_row);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          old_range.take(i, sizeof(C) == 1
+                                ? widen_e4m3(reinterpret_cast<const uint16_t*>(&x)[i])
+                                : reinterpret_cast<const uint32_t*>(&x)[i]);
+      }
+      const T* fresh = k + (te - re) * p.k_token;  // of the page's row 0, were it new
+#pragma unroll 8
+      for (int r = begin + sub; r <= re; r += ROWS) {
+        const Eight<T> x = *reinterpret_cast<const Eight<T>*>(fresh + r * p.k_token);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          new_range.take(i, reinterpret_cast<const uint32_t*>(&x)[i]);
+      }
+    }
+    float lo[8], hi[8];
+    {
+      const Eight<C> new_lo =
+          rounded<T, C>(*reinterpret_cast<const Eight<T>*>(new_range.lo), p.k_inverse);
+      const Eight<C> new_hi =
+          rounded<T, C>(*reinterpret_cast<const Eight<T>*>(new_range.hi), p.k_inverse);
+      const Old* old_lo = reinterpret_cast<const Old*>(old_range.lo);
+      const Old* old_hi = reinterpret_cast<const Old*>(old_range.hi);
+      const T* raw_lo = reinterpret_cast<const T*>(new_range.lo);
+      const T* raw_hi = reinterpret_cast<const T*>(new_range.hi);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        lo[i] = to_float(old_lo[i]), hi[i] = to_float(old_hi[i]);
+        if (to_float(raw_lo[i]) <= to_float(raw_hi[i])) {  // some new row is not NaN
+          lo[i] = fminf(lo[i], to_float(new_lo.x[i]));
+          hi[i] = fmaxf(hi[i], to_float(new_hi.x[i]));
+        }
+      }
     }
     float top = 0.0f;
 #pragma unroll

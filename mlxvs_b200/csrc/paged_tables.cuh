@@ -16,6 +16,7 @@ namespace mlxvs_b200 {
 
 constexpr int TABLES_THREADS = 256;
 constexpr int TABLES_TOKENS = 2048;  // tokens of one block
+constexpr int TABLES_UNROLL = 4;     // tokens of one thread at a time
 
 struct TablesParams {
   const int32_t *past, *fresh;
@@ -53,6 +54,8 @@ __device__ __forceinline__ int3 block_scan3(int3 v, int3* warp_sums, int3* total
   return make_int3(v.x + before.x, v.y + before.y, v.z + before.z);
 }
 
+// ITEMS: requests of one thread at a time.
+template <int ITEMS>
 __global__ void __launch_bounds__(TABLES_THREADS) paged_tables_kernel(const TablesParams p) {
   __shared__ int3 warp_sums[TABLES_THREADS / 32];
   __shared__ int4 met[TABLES_TOKENS];  // first token, past, request, page base
@@ -66,43 +69,65 @@ __global__ void __launch_bounds__(TABLES_THREADS) paged_tables_kernel(const Tabl
   __syncthreads();
   int2 base = make_int2(0, 0);  // tokens and pages of the requests before
   int count = 0;                // requests met so far
-  for (int64_t r0 = 0; r0 < p.requests && (writer || base.x < t1); r0 += TABLES_THREADS) {
-    const int64_t r = r0 + threadIdx.x;
-    int past = 0, fresh = 0, need = 0, b0 = 0;
-    if (r < p.requests) {
-      past = max(p.past[r], 0);
-      fresh = max(p.fresh[r], 0);
-      b0 = (int)p.page.div((uint32_t)past + P - 1);
-      const int b1 = min((int)p.page.div((uint32_t)past + fresh + P - 1), (int)p.width);
-      need = max(b1 - b0, 0);
+  for (int64_t r0 = 0; r0 < p.requests && (writer || base.x < t1);
+       r0 += TABLES_THREADS * ITEMS) {
+    // a few requests per thread, in order
+    int past[ITEMS], fresh[ITEMS], need[ITEMS], b0[ITEMS];
+    int3 mine = make_int3(0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int64_t r = r0 + threadIdx.x * ITEMS + i;
+      past[i] = fresh[i] = 0;
+      if (r < p.requests) past[i] = max(p.past[r], 0), fresh[i] = max(p.fresh[r], 0);
+    }
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      b0[i] = (int)p.page.div((uint32_t)past[i] + P - 1);
+      const int b1 = min((int)p.page.div((uint32_t)past[i] + fresh[i] + P - 1), (int)p.width);
+      need[i] = max(b1 - b0[i], 0);
+      mine.x += fresh[i], mine.y += need[i];
     }
     int3 total;
-    int3 sum = block_scan3(make_int3(fresh, need, 0), warp_sums, &total);
-    const int start = base.x + sum.x - fresh, off = base.y + sum.y - need;
+    int3 sum = block_scan3(mine, warp_sums, &total);
+    int start = base.x + sum.x - mine.x, off = base.y + sum.y - mine.y;
     const bool range_meets = base.x < t1 && base.x + total.x > t0;
     base.x += total.x, base.y += total.y;
+    int at = count;
     if (range_meets) {
       // some request of these may meet the block's tokens: keep those, in order
-      const int meets = fresh > 0 && start < t1 && start + fresh > t0;
+      int meets = 0, first = start;
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        meets += fresh[i] > 0 && first < t1 && first + fresh[i] > t0;
+        first += fresh[i];
+      }
       sum = block_scan3(make_int3(meets, 0, 0), warp_sums, &total);
-      if (meets) met[count + sum.x - 1] = make_int4(start, past, (int)r, off - b0);
+      at += sum.x - meets;
       count += total.x;
     }
-    if (writer && r < p.requests) {
-      p.starts[r] = start;
-      if (fresh > 0) {
-        // tokens that get no slot: past the table's width, past the end of
-        // the free list, or in a begun page that the table does not hold
-        const int64_t avail = max((int64_t)0, min((int64_t)need, p.num_free - off));
-        const int end = past + fresh;
-        const int64_t held = min(min((int64_t)end, (b0 + avail) * P), (int64_t)width_tokens);
-        int64_t lost = end - max(held, (int64_t)min(past, end));
-        const int begun = past % P == 0 ? 0 : min(fresh, P - past % P);
-        if (begun > 0 && past < width_tokens &&
-            p.table[r * p.width + p.page.div(past)] < 0)
-          lost += begun;
-        if (lost > 0) atomicAdd(&lost_sum, (int)lost);
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int64_t r = r0 + threadIdx.x * ITEMS + i;
+      if (range_meets && fresh[i] > 0 && start < t1 && start + fresh[i] > t0)
+        met[at++] = make_int4(start, past[i], (int)r, off - b0[i]);
+      if (writer && r < p.requests) {
+        p.starts[r] = start;
+        if (fresh[i] > 0) {
+          // tokens that get no slot: past the table's width, past the end of
+          // the free list, or in a begun page that the table does not hold
+          const int64_t avail = max((int64_t)0, min((int64_t)need[i], p.num_free - off));
+          const int end = past[i] + fresh[i];
+          const int64_t held =
+              min(min((int64_t)end, (b0[i] + avail) * P), (int64_t)width_tokens);
+          int64_t lost = end - max(held, (int64_t)past[i]);
+          const int begun = past[i] % P == 0 ? 0 : min(fresh[i], P - past[i] % P);
+          if (begun > 0 && past[i] < width_tokens &&
+              p.table[r * p.width + p.page.div(past[i])] < 0)
+            lost += begun;
+          if (lost > 0) atomicAdd(&lost_sum, (int)lost);
+        }
       }
+      start += fresh[i], off += need[i];
     }
   }
   __syncthreads();
@@ -111,36 +136,49 @@ __global__ void __launch_bounds__(TABLES_THREADS) paged_tables_kernel(const Tabl
     p.used[0] = base.y;
     p.used[1] = lost_sum;
   }
-  for (int t = t0 + threadIdx.x; t < t1; t += TABLES_THREADS) {
-    // the last request met that starts at or before t
-    int lo = 0, hi = count;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (met[mid].x <= t) lo = mid + 1;
-      else hi = mid;
-    }
-    const int4 m = lo > 0 ? met[lo - 1] : make_int4(-1, 0, -1, 0);
-    int length = 0;
-    int64_t slot = -1;
-    if (t < base.x && m.x >= 0) {
-      const int pos = m.y + (t - m.x);
-      length = pos + 1;
-      if (pos < width_tokens) {
-        const int b = (int)p.page.div(pos), in = pos - b * P;
-        int32_t page;
-        if (b * P >= m.y) {  // handed out in this step
-          const int64_t i = (int64_t)m.w + b;
-          page = i < p.num_free ? p.free_pages[i] : -1;
-          if (in == 0) p.table[(int64_t)m.z * p.width + b] = page;
+  for (int u0 = t0 + threadIdx.x; u0 < t1; u0 += TABLES_THREADS * TABLES_UNROLL) {
+    int row[TABLES_UNROLL], length[TABLES_UNROLL], in[TABLES_UNROLL];
+    int64_t entry[TABLES_UNROLL];  // of the table, to be filled (-1: none)
+    int32_t page[TABLES_UNROLL];
+#pragma unroll
+    for (int u = 0; u < TABLES_UNROLL; ++u) {
+      const int t = u0 + u * TABLES_THREADS;
+      // the last request met that starts at or before t
+      int lo = 0, hi = t < t1 ? count : 0;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (met[mid].x <= t) lo = mid + 1;
+        else hi = mid;
+      }
+      row[u] = -1, length[u] = 0, page[u] = -1;
+      if (t < t1 && t < base.x && lo > 0) {
+        const int4 m = met[lo - 1];
+        const int pos = m.y + (t - m.x);
+        row[u] = m.z, length[u] = pos + 1;
+        if (pos < width_tokens) {
+          const int b = (int)p.page.div(pos);
+          in[u] = pos - b * P;
+          const bool fresh = b * P >= m.y;  // handed out in this step
+          const int64_t place = (int64_t)m.z * p.width + b, listed = (int64_t)m.w + b;
+          if (!fresh) page[u] = p.table[place];
+          else if (listed < p.num_free) page[u] = p.free_pages[listed];
+          entry[u] = fresh && in[u] == 0 ? place : -1;
         } else {
-          page = p.table[(int64_t)m.z * p.width + b];
+          in[u] = 0, entry[u] = -1;
         }
-        if (page >= 0) slot = (int64_t)page * P + in;
+      } else {
+        in[u] = 0, entry[u] = -1;
       }
     }
-    p.token_requests[t] = length > 0 ? m.z : -1;
-    p.lengths[t] = length;
-    p.slots[t] = slot;
+#pragma unroll
+    for (int u = 0; u < TABLES_UNROLL; ++u) {
+      const int t = u0 + u * TABLES_THREADS;
+      if (t >= t1) break;
+      if (entry[u] >= 0) p.table[entry[u]] = page[u];  // a new page's first token
+      p.token_requests[t] = row[u];
+      p.lengths[t] = length[u];
+      p.slots[t] = page[u] >= 0 ? (int64_t)page[u] * P + in[u] : -1;
+    }
   }
 }
 
