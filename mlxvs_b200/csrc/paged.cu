@@ -20,6 +20,13 @@ constexpr int MAX_DIM = 256;
 constexpr int MAX_PAGE = 1024;
 constexpr int MAX_SELECTED = 256;
 
+// Argument checks: the message is only put together when one fails (a call's
+// checks would otherwise take longer than its launch).
+#define REQUIRE(ok, msg)                                          \
+  do {                                                            \
+    if (!(ok)) throw std::invalid_argument(std::string(op) + (msg)); \
+  } while (0)
+
 int type_size(int type) { return type == MLXVS_FLOAT8_E4M3 ? 1 : 2; }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -37,60 +44,57 @@ void dispatch_types(int type, int cache_type, F&& f) {
     f(__nv_bfloat16{}, __nv_fp8_e4m3{});
 }
 
-void check_types(const std::string& op, int type, int cache_type) {
-  require(type == MLXVS_FLOAT16 || type == MLXVS_BFLOAT16,
-          op + "queries, keys and values must be float16 or bfloat16.");
-  require(cache_type == type || cache_type == MLXVS_FLOAT8_E4M3,
-          op + "the cache must have their type or be float8_e4m3.");
+void check_types(const char* op, int type, int cache_type) {
+  REQUIRE(type == MLXVS_FLOAT16 || type == MLXVS_BFLOAT16,
+          "queries, keys and values must be float16 or bfloat16.");
+  REQUIRE(cache_type == type || cache_type == MLXVS_FLOAT8_E4M3,
+          "the cache must have their type or be float8_e4m3.");
 }
 
 // Shape, strides and alignment of the cache's tensors.
-void check_cache(const std::string& op, const mlxvs_paged_cache& c, bool rows) {
-  require(c.pages >= 0 && c.pages < (1LL << 31), op + "the number of pages must be in [0, 2^31).");
-  require(c.page_size >= 1 && c.page_size <= MAX_PAGE, op + "page_size must be in [1, 1024].");
-  require(c.heads >= 1 && c.heads <= 65535, op + "the key heads must be in [1, 65535].");
+void check_cache(const char* op, const mlxvs_paged_cache& c, bool rows) {
+  REQUIRE(c.pages >= 0 && c.pages < (1LL << 31), "the number of pages must be in [0, 2^31).");
+  REQUIRE(c.page_size >= 1 && c.page_size <= MAX_PAGE, "page_size must be in [1, 1024].");
+  REQUIRE(c.heads >= 1 && c.heads <= 4096, "the key heads must be in [1, 4096].");
   const int unit = 16 / type_size(c.type);
   const int d_unit = rows ? unit : 8;
-  require(c.dim >= d_unit && c.dim <= MAX_DIM && c.dim % d_unit == 0,
-          op + "the head dimension must be a multiple of " + std::to_string(d_unit) +
-              " and at most 256.");
+  REQUIRE(c.dim >= d_unit && c.dim <= MAX_DIM && c.dim % d_unit == 0,
+          "the head dimension must be a multiple of " + std::to_string(d_unit) +
+                                " and at most 256.");
   if (!rows) return;
-  require(c.pages == 0 || (c.keys != nullptr && c.values != nullptr),
-          op + "keys and values must not be NULL.");
-  require(aligned16(c.keys) && aligned16(c.values),
-          op + "keys and values must be 16-byte aligned.");
+  REQUIRE(c.pages == 0 || (c.keys != nullptr && c.values != nullptr),
+          "keys and values must not be NULL.");
+  REQUIRE(aligned16(c.keys) && aligned16(c.values), "keys and values must be 16-byte aligned.");
   for (int64_t s : {c.key_page_stride, c.key_row_stride, c.key_head_stride, c.value_page_stride,
                     c.value_row_stride, c.value_head_stride})
-    require(s >= 0 && s % unit == 0,
-            op + "the cache's strides must be multiples of 16 bytes and not negative.");
-  require(std::isfinite(c.key_scale) && c.key_scale > 0 && std::isfinite(c.value_scale) &&
-              c.value_scale > 0,
-          op + "k_scale and v_scale must be positive and finite.");
-  require(std::isfinite(1.0f / c.key_scale) && std::isfinite(1.0f / c.value_scale),
-          op + "k_scale and v_scale must have finite reciprocals.");
+    REQUIRE(s >= 0 && s % unit == 0,
+            "the cache's strides must be multiples of 16 bytes and not negative.");
+  REQUIRE(std::isfinite(c.key_scale) && c.key_scale > 0 && std::isfinite(c.value_scale) &&
+              c.value_scale > 0, "k_scale and v_scale must be positive and finite.");
+  REQUIRE(std::isfinite(1.0f / c.key_scale) && std::isfinite(1.0f / c.value_scale),
+          "k_scale and v_scale must have finite reciprocals.");
 }
 
-void check_codes(const std::string& op, const mlxvs_paged_cache& c) {
-  require(c.codes != nullptr && c.scales != nullptr, op + "codes and scales must not be NULL.");
-  require(aligned16(c.codes), op + "codes must be 16-byte aligned.");
+void check_codes(const char* op, const mlxvs_paged_cache& c) {
+  REQUIRE(c.codes != nullptr && c.scales != nullptr, "codes and scales must not be NULL.");
+  REQUIRE(aligned16(c.codes), "codes must be 16-byte aligned.");
 }
 
-void check_queries(const std::string& op, const mlxvs_paged_cache& c,
+void check_queries(const char* op, const mlxvs_paged_cache& c,
                    const mlxvs_paged_queries& q) {
   check_types(op, q.type, c.type);
-  require(q.tokens >= 0 && q.tokens < (1LL << 31), op + "the tokens must be in [0, 2^31).");
-  require(q.heads >= 1 && q.heads % c.heads == 0 && q.heads / c.heads <= 128,
-          op + "the query heads must be 1 to 128 times the key heads.");
-  require(q.rows >= 0 && q.rows < (1LL << 31) && q.width >= 0 && q.width < (1LL << 31),
-          op + "the table must be int32 [requests, width].");
-  require(q.tokens == 0 || (q.q != nullptr && q.lengths != nullptr),
-          op + "q and lengths must not be NULL.");
-  require(q.table != nullptr || q.rows * q.width == 0, op + "table must not be NULL.");
-  require(q.requests != nullptr || q.tokens <= q.rows,
-          op + "without requests every token needs a row of the table.");
-  require(aligned16(q.q) && q.token_stride % 8 == 0 && q.head_stride % 8 == 0 &&
-              q.token_stride >= 0 && q.head_stride >= 0,
-          op + "q must be 16-byte aligned, with strides of multiples of 16 bytes.");
+  REQUIRE(q.tokens >= 0 && q.tokens < (1LL << 31), "the tokens must be in [0, 2^31).");
+  REQUIRE(q.heads >= 1 && q.heads % c.heads == 0 && q.heads / c.heads <= 128,
+          "the query heads must be 1 to 128 times the key heads.");
+  REQUIRE(q.rows >= 0 && q.rows < (1LL << 31) && q.width >= 0 && q.width < (1LL << 31),
+          "the table must be int32 [requests, width].");
+  REQUIRE(q.tokens == 0 || (q.q != nullptr && q.lengths != nullptr),
+          "q and lengths must not be NULL.");
+  REQUIRE(q.table != nullptr || q.rows * q.width == 0, "table must not be NULL.");
+  REQUIRE(q.requests != nullptr || q.tokens <= q.rows,
+          "without requests every token needs a row of the table.");
+  REQUIRE(aligned16(q.q) && q.token_stride % 8 == 0 && q.head_stride % 8 == 0 &&
+              q.token_stride >= 0 && q.head_stride >= 0, "q must be 16-byte aligned, with strides of multiples of 16 bytes.");
 }
 
 // More than 48 KB of shared memory, with the kernel's static arrays (at most 16
@@ -106,12 +110,24 @@ void allow_smem(K* kernel, size_t bytes) {
 template <class T, class C, int DP, int NT>
 void launch_attention(AttentionParams p, DeviceInfo& dev, Scratch& scratch, cudaStream_t s) {
   using S = AttentionShape<T, C, DP, NT>;
-  const int blocks = dev.sms * S::BLOCKS;
-  p.cut = scratch.alloc<int4>(blocks + ((size_t)blocks * 2 * S::PART + 3) / 4);
-  p.part = reinterpret_cast<float*>(p.cut + blocks);
   auto* kernel = p.selected ? paged_attention_kernel<T, C, DP, NT, true>
                             : paged_attention_kernel<T, C, DP, NT, false>;
   allow_smem(kernel, S::SMEM);
+  // Rows of few tiles are not cut: a block each, and no second kernel.  Longest
+  // possible rows of 8 tiles: two requests of up to 300 keys 8.1 -> 5.6 us, and
+  // 415 tokens with 9 pages of 24 20 -> 14 us.
+  const int64_t keys = (p.selected ? (int64_t)p.n : p.width) * p.page.d;
+  const int64_t all = p.tokens * p.heads * ((p.group + S::HEADS - 1) / S::HEADS);
+  if (keys <= 8 * S::KEYS && all < (1LL << 31)) {
+    p.whole = 1;
+    ProfScope prof("paged_attention", s);
+    kernel<<<(unsigned)all, S::WARPS * 32, S::SMEM, s>>>(p);
+    CK(cudaGetLastError());
+    return;
+  }
+  const int blocks = dev.sms * S::BLOCKS;
+  p.cut = scratch.alloc<int4>(blocks + ((size_t)blocks * 2 * S::PART + 3) / 4);
+  p.part = reinterpret_cast<float*>(p.cut + blocks);
   {
     ProfScope prof("paged_attention", s);
     kernel<<<blocks, S::WARPS * 32, S::SMEM, s>>>(p);
@@ -204,21 +220,20 @@ void paged_tables(const int32_t* past, const int32_t* fresh, int64_t requests, i
                   const int32_t* free_pages, int64_t num_free, int32_t* table, int64_t width,
                   int64_t num_tokens, int32_t* starts, int32_t* token_requests,
                   int32_t* lengths, int64_t* slots, int32_t* used, cudaStream_t s) {
-  const std::string op = "[mlxvs::paged_tables] ";
-  require(requests >= 0 && requests < (1LL << 31), op + "the requests must be in [0, 2^31).");
-  require(page_size >= 1 && page_size <= MAX_PAGE, op + "page_size must be in [1, 1024].");
-  require(num_tokens >= 0 && num_tokens < (1LL << 31) - TABLES_TOKENS,
-          op + "num_tokens must be in [0, 2^31).");
-  require(num_free >= 0 && width >= 0 && width < (1LL << 31),
-          op + "the table must be int32 [requests, width].");
-  require(requests == 0 || (past != nullptr && fresh != nullptr),
-          op + "past and fresh must not be NULL.");
-  require(requests * width == 0 || table != nullptr, op + "table must not be NULL.");
-  require(num_free == 0 || free_pages != nullptr, op + "free_pages must not be NULL.");
-  require(starts != nullptr && used != nullptr &&
+  const char* op = "[mlxvs::paged_tables] ";
+  REQUIRE(requests >= 0 && requests < (1LL << 31), "the requests must be in [0, 2^31).");
+  REQUIRE(page_size >= 1 && page_size <= MAX_PAGE, "page_size must be in [1, 1024].");
+  REQUIRE(num_tokens >= 0 && num_tokens < (1LL << 31) - TABLES_TOKENS,
+          "num_tokens must be in [0, 2^31).");
+  REQUIRE(num_free >= 0 && width >= 0 && width < (1LL << 31),
+          "the table must be int32 [requests, width].");
+  REQUIRE(requests == 0 || (past != nullptr && fresh != nullptr),
+          "past and fresh must not be NULL.");
+  REQUIRE(requests * width == 0 || table != nullptr, "table must not be NULL.");
+  REQUIRE(num_free == 0 || free_pages != nullptr, "free_pages must not be NULL.");
+  REQUIRE(starts != nullptr && used != nullptr &&
               (num_tokens == 0 ||
-               (token_requests != nullptr && lengths != nullptr && slots != nullptr)),
-          op + "outputs must not be NULL.");
+               (token_requests != nullptr && lengths != nullptr && slots != nullptr)), "outputs must not be NULL.");
   device_info();
   const TablesParams p{past,  fresh,      requests, FastDiv((uint32_t)page_size), free_pages,
                        num_free, table,  width,    num_tokens, starts, token_requests,
@@ -237,15 +252,15 @@ void paged_tables(const int32_t* past, const int32_t* fresh, int64_t requests, i
 void paged_store(const mlxvs_paged_cache& c, const void* k, const void* v, int type,
                  int64_t tokens, int64_t k_token, int64_t k_head, int64_t v_token,
                  int64_t v_head, const int64_t* slots, cudaStream_t s) {
-  const std::string op = "[mlxvs::paged_store] ";
+  const char* op = "[mlxvs::paged_store] ";
   check_types(op, type, c.type);
   check_cache(op, c, true);
-  require(tokens >= 0 && tokens < (1LL << 31), op + "the tokens must be in [0, 2^31).");
-  require(tokens == 0 || (k != nullptr && v != nullptr && slots != nullptr),
-          op + "k, v and slots must not be NULL.");
-  require(aligned16(k) && aligned16(v), op + "k and v must be 16-byte aligned.");
+  REQUIRE(tokens >= 0 && tokens < (1LL << 31), "the tokens must be in [0, 2^31).");
+  REQUIRE(tokens == 0 || (k != nullptr && v != nullptr && slots != nullptr),
+          "k, v and slots must not be NULL.");
+  REQUIRE(aligned16(k) && aligned16(v), "k and v must be 16-byte aligned.");
   for (int64_t x : {k_token, k_head, v_token, v_head})
-    require(x >= 0 && x % 8 == 0, op + "the strides of k and v must be multiples of 16 bytes.");
+    REQUIRE(x >= 0 && x % 8 == 0, "the strides of k and v must be multiples of 16 bytes.");
   if (c.codes != nullptr || c.scales != nullptr) check_codes(op, c);
   DeviceInfo& dev = device_info();
   if (tokens == 0 || c.pages == 0) return;
@@ -275,19 +290,19 @@ void paged_store(const mlxvs_paged_cache& c, const void* k, const void* v, int t
 
 void paged_select(const mlxvs_paged_cache& c, const mlxvs_paged_queries& q, int n, int first,
                   int last, int32_t* pages, cudaStream_t s) {
-  const std::string op = "[mlxvs::paged_select] ";
+  const char* op = "[mlxvs::paged_select] ";
   check_cache(op, c, false);
   check_codes(op, c);
   check_queries(op, c, q);
-  require(n >= 1 && n <= MAX_SELECTED, op + "n must be in [1, 256].");
-  require(first >= 0 && last >= 0 && first + last <= n,
-          op + "first and last must be at least 0 and together at most n.");
-  require(q.tokens == 0 || pages != nullptr, op + "pages must not be NULL.");
+  REQUIRE(n >= 1 && n <= MAX_SELECTED, "n must be in [1, 256].");
+  REQUIRE(first >= 0 && last >= 0 && first + last <= n,
+          "first and last must be at least 0 and together at most n.");
+  REQUIRE(q.tokens == 0 || pages != nullptr, "pages must not be NULL.");
   DeviceInfo& dev = device_info();
   // keys of one token and the static arrays must fit a block's shared memory
   const int64_t room = (dev.max_smem - 16384) / 4;
-  require(q.width <= room,
-          op + "the table must have at most " + std::to_string(room) + " pages a request.");
+  REQUIRE(q.width <= room,
+          "the table must have at most " + std::to_string(room) + " pages a request.");
   if (q.tokens == 0) return;
   int shift = 0;
   while ((1 << shift) < q.heads / c.heads) ++shift;
@@ -332,14 +347,14 @@ void paged_select(const mlxvs_paged_cache& c, const mlxvs_paged_queries& q, int 
 void paged_attention(const mlxvs_paged_cache& c, const mlxvs_paged_queries& q,
                      const int32_t* pages, int n, float scale, void* out, float* lse,
                      cudaStream_t s) {
-  const std::string op = "[mlxvs::paged_attention] ";
+  const char* op = "[mlxvs::paged_attention] ";
   check_cache(op, c, true);
   check_queries(op, c, q);
-  require(pages == nullptr || (n >= 1 && n <= (1 << 20)),
-          op + "pages must be int32 [tokens, key heads, n], n at most 2^20.");
-  require(std::isfinite(scale), op + "scale must be finite.");
-  require(q.tokens == 0 || out != nullptr, op + "out must not be NULL.");
-  require(aligned16(out), op + "out must be 16-byte aligned.");
+  REQUIRE(pages == nullptr || (n >= 1 && n <= (1 << 20)),
+          "pages must be int32 [tokens, key heads, n], n at most 2^20.");
+  REQUIRE(std::isfinite(scale), "scale must be finite.");
+  REQUIRE(q.tokens == 0 || out != nullptr, "out must not be NULL.");
+  REQUIRE(aligned16(out), "out must be 16-byte aligned.");
   DeviceInfo& dev = device_info();
   if (q.tokens == 0) return;
   const float log2e = 1.44269504088896f;
@@ -348,7 +363,7 @@ void paged_attention(const mlxvs_paged_cache& c, const mlxvs_paged_queries& q,
                     c.key_head_stride, c.value_page_stride, c.value_row_stride,
                     c.value_head_stride, c.pages, FastDiv((uint32_t)c.page_size), q.table,
                     q.rows, q.width, q.requests, q.lengths, pages, n, scale * c.key_scale * log2e,
-                    c.value_scale, out, lse, nullptr, nullptr};
+                    c.value_scale, out, lse, nullptr, nullptr, 0};
   Scratch scratch(s);
   dispatch_types(q.type, c.type, [&](auto t, auto ct) {
     auto shaped = [&](auto dp, auto nt) {

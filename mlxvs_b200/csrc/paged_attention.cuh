@@ -35,6 +35,7 @@ struct AttentionParams {
   float* lse;            // [tokens, heads * group] or null
   float* part;           // [blocks][2][8 NT heads][DP + 2]: sums, maximum, sum
   int4* cut;             // [blocks]: the row that the block's start cuts
+  int whole;             // a row for each block, none cut
 };
 
 // ------------------------------------------------------------------ PTX
@@ -228,7 +229,12 @@ __global__ void __launch_bounds__(AttentionShape<T, C, DP, NT>::WARPS * 32,
   int64_t total;
   int64_t x, x1, per;
   AttentionRow row;
-  if (SPARSE) {
+  if (p.whole) {
+    row.t = blockIdx.x / per_token;
+    row.h = (int)(blockIdx.x % per_token) / chunks, row.chunk = (int)(blockIdx.x % per_token) % chunks;
+    row.tiles = tiles_of(row.t);
+    row.start = x = 0, x1 = per = row.tiles;
+  } else if (SPARSE) {
     row.tiles = tiles_of(0);
     const int places = row.tiles + ROW_COST;
     total = p.tokens * per_token * places;
@@ -284,7 +290,7 @@ __global__ void __launch_bounds__(AttentionShape<T, C, DP, NT>::WARPS * 32,
   // the block's first tile, and how many places are left from there: a range
   // that ends within a row's cost leaves the row to the next block
   const bool cut = x < x1 && x > row.start;
-  if (tid == 0) {
+  if (tid == 0 && !p.whole) {
     // a row that this block's start cuts, listed by the first block that cuts it
     const bool first = cut && row.start >= x - per;
     const int64_t last = first ? (row.start + row.tiles - 1) / per : 0;

@@ -20,6 +20,7 @@ import collections
 import struct
 
 import torch
+from torch import Tensor, float32, int8, int32, int64
 
 from . import _check, _load
 
@@ -49,16 +50,17 @@ def _type(t, op, name):
 def _want(t, op, name, dtype, dim, index):
     """Checks for a contiguous tensor of the given type and number of
     dimensions on the CUDA device `index`."""
-    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.dim() == dim
-            and t.is_contiguous() and t.is_cuda):
-        raise ValueError(f"[{op}] {name} must be a contiguous {dim}-D CUDA tensor of {dtype}.")
-    if t.get_device() != index:
+    if (isinstance(t, Tensor) and t.dtype is dtype and t.dim() == dim and t.is_contiguous()
+            and t.get_device() == index):
+        return
+    if isinstance(t, Tensor) and t.is_cuda and t.get_device() != index:
         raise ValueError(f"[{op}] {name} must be on cuda:{index}.")
+    raise ValueError(f"[{op}] {name} must be a contiguous {dim}-D CUDA tensor of {dtype}.")
 
 
 def _rows(t, op, name, dims):
     """The strides of a CUDA tensor with a contiguous last dimension."""
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == len(dims)):
+    if not (isinstance(t, Tensor) and t.is_cuda and t.dim() == len(dims)):
         raise ValueError(f"[{op}] {name} must be a CUDA tensor [{', '.join(dims)}].")
     strides = t.stride()
     if strides[-1] != 1 and t.shape[-1] > 1:
@@ -67,8 +69,8 @@ def _rows(t, op, name, dims):
 
 
 def _bounds(codes, scales, op, pages, heads, dim, index):
-    _want(codes, op, "codes", torch.int8, 4, index)
-    _want(scales, op, "scales", torch.float32, 2, index)
+    _want(codes, op, "codes", int8, 4, index)
+    _want(scales, op, "scales", float32, 2, index)
     if codes.shape != (pages, heads, 2, dim) or scales.shape != (pages, heads):
         raise ValueError(f"[{op}] codes must be [pages, key heads, 2, dim] and scales "
                          "[pages, key heads].")
@@ -103,15 +105,15 @@ def _queries(q, table, lengths, requests, op):
     """mlxvs_paged_queries of the tensors, q's shape and its device."""
     qs = _rows(q, op, "q", _Q_DIMS)
     index = q.get_device()
-    _want(table, op, "table", torch.int32, 2, index)
-    _want(lengths, op, "lengths", torch.int32, 1, index)
+    _want(table, op, "table", int32, 2, index)
+    _want(lengths, op, "lengths", int32, 1, index)
     shape = q.shape
     tokens = shape[0]
     if lengths.shape[0] != tokens:
         raise ValueError(f"[{op}] lengths must be [tokens].")
     at_requests = 0
     if requests is not None:
-        _want(requests, op, "requests", torch.int32, 1, index)
+        _want(requests, op, "requests", int32, 1, index)
         if requests.shape[0] != tokens:
             raise ValueError(f"[{op}] requests must be [tokens].")
         at_requests = requests.data_ptr()
@@ -127,8 +129,7 @@ def _call(function, args, index, stream):
         handle = _current_stream(index)
     else:
         handle = stream if isinstance(stream, int) else stream.cuda_stream
-    before = _current_device()
-    if before == index:
+    if _current_device() == index:
         rc = function(*args, handle)
     else:
         with torch.cuda.device(index):
@@ -155,20 +156,20 @@ def paged_tables(past, fresh, table, free_pages, page_size, num_tokens, *, strea
     """
     op = "mlxvs::paged_tables"
     lib = _load()
-    if not (isinstance(past, torch.Tensor) and past.is_cuda):
+    if not (isinstance(past, Tensor) and past.is_cuda):
         raise ValueError(f"[{op}] past must be a contiguous 1-D CUDA tensor of torch.int32.")
     index = past.get_device()
-    _want(past, op, "past", torch.int32, 1, index)
-    _want(fresh, op, "fresh", torch.int32, 1, index)
-    _want(table, op, "table", torch.int32, 2, index)
-    _want(free_pages, op, "free_pages", torch.int32, 1, index)
+    _want(past, op, "past", int32, 1, index)
+    _want(fresh, op, "fresh", int32, 1, index)
+    _want(table, op, "table", int32, 2, index)
+    _want(free_pages, op, "free_pages", int32, 1, index)
     requests, num_tokens = past.shape[0], int(num_tokens)
     rows, width = table.shape
     if fresh.shape[0] != requests or rows != requests:
         raise ValueError(f"[{op}] past, fresh and table must have one row per request.")
     if num_tokens < 0:
         raise ValueError(f"[{op}] num_tokens must be in [0, 2^31).")
-    slots = past.new_empty(num_tokens, dtype=torch.int64)
+    slots = past.new_empty(num_tokens, dtype=int64)
     ints = past.new_empty(2 * num_tokens + requests + 3)
     at = ints.data_ptr()
     starts = at + 8 * num_tokens
@@ -199,7 +200,7 @@ def paged_store(k, v, slots, keys, values, codes=None, scales=None, *, k_scale=1
     if k.shape[1:] != shape[2:]:
         raise ValueError(f"[{op}] k and v must have the cache's heads and dimension.")
     tokens = k.shape[0]
-    _want(slots, op, "slots", torch.int64, 1, index)
+    _want(slots, op, "slots", int64, 1, index)
     if slots.shape[0] != tokens:
         raise ValueError(f"[{op}] slots must be [tokens].")
     _call(lib.mlxvs_paged_store_device,
@@ -223,7 +224,7 @@ def paged_select(q, codes, scales, table, lengths, page_size, n, *, requests=Non
     lib = _load()
     n = int(n)
     queries, shape, index = _queries(q, table, lengths, requests, op)
-    if not (isinstance(codes, torch.Tensor) and codes.dim() == 4):
+    if not (isinstance(codes, Tensor) and codes.dim() == 4):
         raise ValueError(f"[{op}] codes must be [pages, key heads, 2, dim] and scales "
                          "[pages, key heads].")
     pages, heads = codes.shape[:2]
@@ -255,7 +256,7 @@ def paged_attention(q, keys, values, table, lengths, *, requests=None, pages=Non
         raise ValueError(f"[{op}] q must have the cache's dimension.")
     n = at_pages = 0
     if pages is not None:
-        _want(pages, op, "pages", torch.int32, 3, index)
+        _want(pages, op, "pages", int32, 3, index)
         tokens, heads, n = pages.shape
         if tokens != shape[0] or heads != kv[2] or n < 1:
             raise ValueError(f"[{op}] pages must be [tokens, key heads, n].")
@@ -263,7 +264,7 @@ def paged_attention(q, keys, values, table, lengths, *, requests=None, pages=Non
     if scale is None:
         scale = shape[2] ** -0.5
     out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
-    lse = q.new_empty(shape[:2], dtype=torch.float32) if return_lse else None
+    lse = q.new_empty(shape[:2], dtype=float32) if return_lse else None
     _call(lib.mlxvs_paged_attention_device,
           (cache, queries, at_pages, n, scale, out.data_ptr(),
            lse.data_ptr() if return_lse else None), index, stream)
