@@ -530,3 +530,22 @@ def test_a_step_on_another_stream_and_in_a_graph():
         torch.cuda.synchronize()
         check(*got)
     mv.synchronize()
+
+
+@pytest.mark.parametrize("cache", ["bf16", "e4m3"])
+def test_example(cache):
+    """The decoding example: with all pages selected the sparse attention is
+    the whole one; with few, part of its weight."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples",
+                        "paged_decode.py")
+    spec = importlib.util.spec_from_file_location("paged_decode", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    few = example.run(requests=5, steps=3, passage_tokens=100, pages_seen=3, cache=cache)
+    assert len(few) == 4 and all(0.1 < s < 1.0 for s in few)
+    every = example.run(requests=5, steps=3, passage_tokens=100, pages_seen=16, cache=cache)
+    # both sum the same weights, in another order: float32 roundings
+    assert all(abs(s - 1.0) < 1e-4 for s in every)
