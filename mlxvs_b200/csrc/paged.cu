@@ -114,8 +114,9 @@ void launch_attention(AttentionParams p, DeviceInfo& dev, Scratch& scratch, cuda
                             : paged_attention_kernel<T, C, DP, NT, false>;
   allow_smem(kernel, S::SMEM);
   // Rows of few tiles are not cut: a block each, and no second kernel.  Longest
-  // possible rows of 8 tiles: two requests of up to 300 keys 8.1 -> 5.6 us, and
-  // 415 tokens with 9 pages of 24 20 -> 14 us.
+  // possible rows of 8 tiles: two requests of up to 300 keys 8.1 -> 6.0 us in a
+  // graph (and one launch less on the host), 415 tokens with 9 pages of 24 and
+  // their selection 31.3 -> 30.0 us.
   const int64_t keys = (p.selected ? (int64_t)p.n : p.width) * p.page.d;
   const int64_t all = p.tokens * p.heads * ((p.group + S::HEADS - 1) / S::HEADS);
   if (keys <= 8 * S::KEYS && all < (1LL << 31)) {
@@ -175,6 +176,8 @@ CUtensorMap cache_map(const void* base, const AttentionParams& p, int64_t head_s
 // Whether selected pages are walked by tiles of tokens: prompts (more tokens
 // than requests) with enough tiles for the SMs, and a cache that a tensor map
 // can describe.  Pages of under 16 rows would leave most of a stage empty.
+// 5,229 tokens with 16 pages of 64: 672 us by tiles, 1423 by rows of their own
+// pages (10.7 GB from L2, 7.5 TB/s).
 template <class T, class C, int DP>
 bool prompt_tiles(const AttentionParams& p, const DeviceInfo& dev) {
   using S = PromptShape<T, C, DP>;
@@ -270,9 +273,10 @@ void paged_store(const mlxvs_paged_cache& c, const void* k, const void* v, int t
                 c.pages, FastDiv((uint32_t)c.page_size), c.heads, c.dim,
                 1.0f / c.key_scale, 1.0f / c.value_scale, c.codes, c.scales};
   // Chunks of one token while that fills the GPU (single tokens end a page's
-  // rows each, so a chunk of them would go one after another), 32 at most.
+  // rows each, so a chunk of them would go one after another), 16 at most (of 4, 8, 16 and 32: 28.9, 24.0, 23.7 and 27.4 us
+  // for 13,881 tokens).
   const int64_t chunk =
-      std::max<int64_t>(1, std::min<int64_t>(32, tokens * c.heads / (dev.sms * 16)));
+      std::max<int64_t>(1, std::min<int64_t>(16, tokens * c.heads / (dev.sms * 16)));
   const dim3 grid((unsigned)((tokens + chunk - 1) / chunk),
                   (c.heads + STORE_WARPS - 1) / STORE_WARPS);
   ProfScope prof("paged_store", s);
@@ -312,7 +316,9 @@ void paged_select(const mlxvs_paged_cache& c, const mlxvs_paged_queries& q, int 
                        n, first, last, pages};
   // Prompts (more tokens than requests) share the pages' codes between 8 tokens
   // of a tile; single tokens have pages of their own.  Clusters share the pages
-  // of few tiles among more SMs.
+  // of few tiles among more SMs: 7 requests of up to 250,000 keys took 91 us
+  // without clusters and 33 with up to 8 blocks, 256 rows of up to 500 pages 23
+  // us without and 31 with 4.
   const bool tiles = q.tokens > q.rows && 8 * q.width <= room;
   const int64_t units = (q.tokens + (tiles ? 7 : 0)) / (tiles ? 8 : 1);
   int cluster = 1;

@@ -10,6 +10,15 @@
 // selected it.  As in paged_attention.cuh the products are transposed
 // (S^T = K Q^T, O^T = V^T P^T): a token's query heads are the 8 columns, so no
 // work is spent on tokens that did not select the page.
+//
+// Bound: 5,229 tokens with 16 of up to 230 pages of 64 each (bf16, 4 key heads of
+// 8, 89 GFLOP) take 672 us, 133 TFLOP/s.  The loads alone take 298 us (the tiles
+// still read 2.5 GB from L2), the products at the warp instructions' full rate
+// would take 257; the rest is the products' latency (a warp has work at one page
+// in four) and the wait for the slowest warp of a stage.  128-row tensor core
+// tiles would multiply every token by every page of the tile: with pages chosen
+// alike they would win, with pages chosen by chance they do eight times the
+// work.
 #pragma once
 
 #include <type_traits>
@@ -63,7 +72,7 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, u
 //
 // The bodies are kept short on purpose: the warps are at different pages at
 // any time, and a body unrolled over a whole page made them wait for
-// instructions more than for anything else.  Two independent tiles (of keys,
+// instructions more than for anything else (2.2 ms in all instead of 0.67).  Two independent tiles (of keys,
 // or of column groups) are in flight in each, to cover the latency of the chain
 // products -> weights -> products.
 template <class T, class C, int DP, int NT, int WHICH, int MT>

