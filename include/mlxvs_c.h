@@ -408,7 +408,8 @@ typedef struct {
  * (at least their number; the tokens past it are padding, so that a
  * captured step can keep its size): token_requests (-1 for padding), lengths
  * (the token's position + 1: the keys it sees; 0 for padding) and slots
- * (page * page_size + row in the page, -1 where it gets none).  starts
+ * (page * page_size + row in the page, -1 where it gets none).  Lengths and
+ * the sum of fresh must stay below 2^31.  starts
  * [requests + 1]: the requests' first tokens.  used[0]: pages asked of
  * free_pages (the next step's list starts behind them), used[1]: new tokens
  * that got no slot, because free_pages ended (their table entries are then

@@ -65,9 +65,13 @@ void check_cache(const char* op, const mlxvs_paged_cache& c, bool rows) {
   REQUIRE(c.pages == 0 || (c.keys != nullptr && c.values != nullptr),
           "keys and values must not be NULL.");
   REQUIRE(aligned16(c.keys) && aligned16(c.values), "keys and values must be 16-byte aligned.");
-  for (int64_t s : {c.key_page_stride, c.key_row_stride, c.key_head_stride, c.value_page_stride,
-                    c.value_row_stride, c.value_head_stride})
-    REQUIRE(s >= 0 && s % unit == 0,
+  // a dimension of one element may have any stride
+  const int64_t strides[6][2] = {
+      {c.pages, c.key_page_stride},   {c.page_size, c.key_row_stride},
+      {c.heads, c.key_head_stride},   {c.pages, c.value_page_stride},
+      {c.page_size, c.value_row_stride}, {c.heads, c.value_head_stride}};
+  for (const auto& s : strides)
+    REQUIRE(s[0] <= 1 || (s[1] >= 0 && s[1] % unit == 0),
             "the cache's strides must be multiples of 16 bytes and not negative.");
   REQUIRE(std::isfinite(c.key_scale) && c.key_scale > 0 && std::isfinite(c.value_scale) &&
               c.value_scale > 0, "k_scale and v_scale must be positive and finite.");
@@ -93,8 +97,10 @@ void check_queries(const char* op, const mlxvs_paged_cache& c,
   REQUIRE(q.table != nullptr || q.rows * q.width == 0, "table must not be NULL.");
   REQUIRE(q.requests != nullptr || q.tokens <= q.rows,
           "without requests every token needs a row of the table.");
-  REQUIRE(aligned16(q.q) && q.token_stride % 8 == 0 && q.head_stride % 8 == 0 &&
-              q.token_stride >= 0 && q.head_stride >= 0, "q must be 16-byte aligned, with strides of multiples of 16 bytes.");
+  REQUIRE(aligned16(q.q) &&
+              (q.tokens <= 1 || (q.token_stride >= 0 && q.token_stride % 8 == 0)) &&
+              (q.heads <= 1 || (q.head_stride >= 0 && q.head_stride % 8 == 0)),
+          "q must be 16-byte aligned, with strides of multiples of 16 bytes.");
 }
 
 // More than 48 KB of shared memory, with the kernel's static arrays (at most 16
@@ -262,8 +268,12 @@ void paged_store(const mlxvs_paged_cache& c, const void* k, const void* v, int t
   REQUIRE(tokens == 0 || (k != nullptr && v != nullptr && slots != nullptr),
           "k, v and slots must not be NULL.");
   REQUIRE(aligned16(k) && aligned16(v), "k and v must be 16-byte aligned.");
-  for (int64_t x : {k_token, k_head, v_token, v_head})
-    REQUIRE(x >= 0 && x % 8 == 0, "the strides of k and v must be multiples of 16 bytes.");
+  for (int64_t x : {k_token, v_token})
+    REQUIRE(tokens <= 1 || (x >= 0 && x % 8 == 0),
+            "the strides of k and v must be multiples of 16 bytes.");
+  for (int64_t x : {k_head, v_head})
+    REQUIRE(c.heads <= 1 || (x >= 0 && x % 8 == 0),
+            "the strides of k and v must be multiples of 16 bytes.");
   if (c.codes != nullptr || c.scales != nullptr) check_codes(op, c);
   DeviceInfo& dev = device_info();
   if (tokens == 0 || c.pages == 0) return;

@@ -123,12 +123,17 @@ def _queries(q, table, lengths, requests, op):
         lengths.data_ptr(), shape[1], _type(q, op, "q")), shape, index
 
 
-def _call(function, args, index, stream):
+def _stream(stream, index):
+    """A context in which `stream` (a torch stream or a cudaStream_t) is the
+    current one, so that outputs are allocated in its order as well."""
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream, device=torch.device("cuda", index))
+    return torch.cuda.stream(stream)
+
+
+def _call(function, args, index):
     """A C entry with the stream as its last argument, on device `index`."""
-    if stream is None:
-        handle = _current_stream(index)
-    else:
-        handle = stream if isinstance(stream, int) else stream.cuda_stream
+    handle = _current_stream(index)
     if _current_device() == index:
         rc = function(*args, handle)
     else:
@@ -159,6 +164,9 @@ def paged_tables(past, fresh, table, free_pages, page_size, num_tokens, *, strea
     if not (isinstance(past, Tensor) and past.is_cuda):
         raise ValueError(f"[{op}] past must be a contiguous 1-D CUDA tensor of torch.int32.")
     index = past.get_device()
+    if stream is not None:
+        with _stream(stream, index):
+            return paged_tables(past, fresh, table, free_pages, page_size, num_tokens)
     _want(past, op, "past", int32, 1, index)
     _want(fresh, op, "fresh", int32, 1, index)
     _want(table, op, "table", int32, 2, index)
@@ -176,7 +184,7 @@ def paged_tables(past, fresh, table, free_pages, page_size, num_tokens, *, strea
     _call(lib.mlxvs_paged_tables_device,
           (past.data_ptr(), fresh.data_ptr(), requests, int(page_size), free_pages.data_ptr(),
            free_pages.shape[0], table.data_ptr(), width, num_tokens, starts, at,
-           at + 4 * num_tokens, slots.data_ptr(), starts + 4 * (requests + 1)), index, stream)
+           at + 4 * num_tokens, slots.data_ptr(), starts + 4 * (requests + 1)), index)
     of, lengths, starts, used = torch.split_with_sizes(
         ints, (num_tokens, num_tokens, requests + 1, 2))
     return PagedTables(starts, of, lengths, slots, used)
@@ -194,6 +202,10 @@ def paged_store(k, v, slots, keys, values, codes=None, scales=None, *, k_scale=1
     ks = _rows(k, op, "k", _K_DIMS)
     vs = _rows(v, op, "v", _K_DIMS)
     index = k.get_device()
+    if stream is not None:
+        with _stream(stream, index):
+            return paged_store(k, v, slots, keys, values, codes, scales, k_scale=k_scale,
+                               v_scale=v_scale)
     cache, shape = _cache(keys, values, codes, scales, k_scale, v_scale, op, index)
     if k.shape != v.shape or k.dtype is not v.dtype or v.get_device() != index:
         raise ValueError(f"[{op}] k and v must have the same shape, type and device.")
@@ -205,7 +217,7 @@ def paged_store(k, v, slots, keys, values, codes=None, scales=None, *, k_scale=1
         raise ValueError(f"[{op}] slots must be [tokens].")
     _call(lib.mlxvs_paged_store_device,
           (cache, k.data_ptr(), v.data_ptr(), _type(k, op, "k"), tokens, ks[0], ks[1], vs[0],
-           vs[1], slots.data_ptr()), index, stream)
+           vs[1], slots.data_ptr()), index)
 
 
 def paged_select(q, codes, scales, table, lengths, page_size, n, *, requests=None, first=1,
@@ -224,6 +236,10 @@ def paged_select(q, codes, scales, table, lengths, page_size, n, *, requests=Non
     lib = _load()
     n = int(n)
     queries, shape, index = _queries(q, table, lengths, requests, op)
+    if stream is not None:
+        with _stream(stream, index):
+            return paged_select(q, codes, scales, table, lengths, page_size, n,
+                                requests=requests, first=first, last=last)
     if not (isinstance(codes, Tensor) and codes.dim() == 4):
         raise ValueError(f"[{op}] codes must be [pages, key heads, 2, dim] and scales "
                          "[pages, key heads].")
@@ -233,7 +249,7 @@ def paged_select(q, codes, scales, table, lengths, page_size, n, *, requests=Non
                         int(page_size), heads, shape[2], _type(q, op, "q"), 1.0, 1.0)
     out = table.new_empty((shape[0], heads, max(n, 0)))
     _call(lib.mlxvs_paged_select_device,
-          (cache, queries, n, int(first), int(last), out.data_ptr()), index, stream)
+          (cache, queries, n, int(first), int(last), out.data_ptr()), index)
     return out
 
 
@@ -251,6 +267,11 @@ def paged_attention(q, keys, values, table, lengths, *, requests=None, pages=Non
     op = "mlxvs::paged_attention"
     lib = _load()
     queries, shape, index = _queries(q, table, lengths, requests, op)
+    if stream is not None:
+        with _stream(stream, index):
+            return paged_attention(q, keys, values, table, lengths, requests=requests,
+                                   pages=pages, scale=scale, k_scale=k_scale, v_scale=v_scale,
+                                   return_lse=return_lse)
     cache, kv = _cache(keys, values, None, None, k_scale, v_scale, op, index)
     if shape[2] != kv[3]:
         raise ValueError(f"[{op}] q must have the cache's dimension.")
@@ -267,5 +288,5 @@ def paged_attention(q, keys, values, table, lengths, *, requests=None, pages=Non
     lse = q.new_empty(shape[:2], dtype=float32) if return_lse else None
     _call(lib.mlxvs_paged_attention_device,
           (cache, queries, at_pages, n, scale, out.data_ptr(),
-           lse.data_ptr() if return_lse else None), index, stream)
+           lse.data_ptr() if return_lse else None), index)
     return (out, lse) if return_lse else out

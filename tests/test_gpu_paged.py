@@ -216,6 +216,8 @@ SELECTED = [
     ([300, 700], [65, 17], 16, 1, 20, 96, 30, "float16", "float8_e4m3fn", "plain"),
     ([4000], [1], 1, 2, 3, 64, 256, "bfloat16", "bfloat16", "plain"),
     ([1500, 1400], [200, 50], 128, 2, 8, 128, 3, "bfloat16", "bfloat16", "plain"),
+    ([300, 31], [33, 31], 8, 2, 4, 8, 6, "float16", "float16", "plain"),
+    ([333], [1], 24, 1, 3, 24, 11, "bfloat16", "bfloat16", "heads first"),
     # enough tokens that tiles of them share the pages
     ([900, 400], [380, 220], 64, 8, 8, 128, 5, "bfloat16", "bfloat16", "plain"),
     ([777, 5, 333], [300, 5, 290], 24, 8, 6, 80, 7, "float16", "float16", "heads first"),
@@ -324,6 +326,45 @@ def test_select_ties_forced_pages_and_odd_queries():
     assert run()[3, 0].tolist() == [0, 1, 2, 3, -1]
     empty = mv.paged_select(q[:0], codes, scales, on_gpu(table), on_gpu(lengths[:0]), page, n)
     assert empty.shape == (0, 1, n)
+
+
+def test_select_of_tokens_in_any_order():
+    """Tokens of several requests and of none, interleaved."""
+    rng = np.random.default_rng(13)
+    tokens, heads, group, dim, page, n = 61, 3, 5, 96, 16, 6
+    codes = np.sort(rng.integers(-127, 128, (70, heads, 2, dim)), 2)
+    scales = 2.0 ** rng.integers(-3, 3, (70, heads))
+    table = rng.integers(-2, 72, (4, 30))  # holes, and pages beyond the cache
+    requests = rng.integers(-1, 5, tokens)
+    lengths = rng.integers(-3, 600, tokens)
+    q = torch_().from_numpy(rng.standard_normal((tokens, heads * group, dim))).cuda().half()
+    got = mv.paged_select(q, on_gpu(codes, "int8"), on_gpu(scales, "float32"), on_gpu(table),
+                          on_gpu(lengths), page, n, requests=on_gpu(requests), first=2, last=2)
+    want = O.paged_select(wide(q), codes, scales, table, lengths, page, n, requests, 2, 2)
+    assert np.array_equal(got.cpu().numpy(), want)
+
+
+def test_strides_of_single_elements_and_given_streams():
+    """A dimension of one element may have any stride; stream= takes a torch
+    stream or a handle."""
+    torch = torch_()
+    rng = np.random.default_rng(14)
+    keys, values = make_cache(rng, 3, 16, 1, 64, "float16")
+    table, lengths = on_gpu([[2, 0, 1]]), on_gpu([40])
+    q = torch.randn(1, 1, 64, device="cuda").half()
+    odd = q.as_strided((1, 1, 64), (3, 5, 1))
+    oddk, oddv = (x.as_strided(x.shape, (x.stride(0), x.stride(1), 7, 1)) for x in (keys, values))
+    want = mv.paged_attention(q, keys, values, table, lengths)
+    assert torch.equal(mv.paged_attention(odd, oddk, oddv, table, lengths), want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for stream in (side, side.cuda_stream):
+        got = mv.paged_attention(q, keys, values, table, lengths, stream=stream)
+        side.synchronize()
+        assert torch.equal(got, want)
+    t = mv.paged_tables(on_gpu([5]), on_gpu([2]), table, on_gpu([1]), 16, 2, stream=side)
+    side.synchronize()
+    assert t.slots.tolist() == [2 * 16 + 5, 2 * 16 + 6]
 
 
 def test_select_many_pages():
