@@ -273,19 +273,20 @@ def paged_attention(q, keys, values, table, lengths, *, requests=None, pages=Non
                                    pages=pages, scale=scale, k_scale=k_scale, v_scale=v_scale,
                                    return_lse=return_lse)
     cache, kv = _cache(keys, values, None, None, k_scale, v_scale, op, index)
-    if shape[2] != kv[3]:
+    tokens, q_heads, dim = shape
+    if dim != kv[3]:
         raise ValueError(f"[{op}] q must have the cache's dimension.")
     n = at_pages = 0
     if pages is not None:
         _want(pages, op, "pages", int32, 3, index)
-        tokens, heads, n = pages.shape
-        if tokens != shape[0] or heads != kv[2] or n < 1:
+        of, heads, n = pages.shape
+        if of != tokens or heads != kv[2] or n < 1:
             raise ValueError(f"[{op}] pages must be [tokens, key heads, n].")
         at_pages = pages.data_ptr()
     if scale is None:
-        scale = shape[2] ** -0.5
+        scale = dim ** -0.5
     out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
-    lse = q.new_empty(shape[:2], dtype=float32) if return_lse else None
+    lse = q.new_empty((tokens, q_heads), dtype=float32) if return_lse else None
     _call(lib.mlxvs_paged_attention_device,
           (cache, queries, at_pages, n, scale, out.data_ptr(),
            lse.data_ptr() if return_lse else None), index)
