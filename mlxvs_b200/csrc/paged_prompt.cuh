@@ -12,10 +12,13 @@
 // work is spent on tokens that did not select the page.
 //
 // Bound: 5,229 tokens with 16 of up to 230 pages of 64 each (bf16, 4 key heads of
-// 8, 89 GFLOP) take 672 us, 133 TFLOP/s.  The loads alone take 298 us (the tiles
-// still read 2.5 GB from L2), the products at the warp instructions' full rate
-// would take 257; the rest is the products' latency (a warp has work at one page
-// in four) and the wait for the slowest warp of a stage.  128-row tensor core
+// 8, 89 GFLOP) take 672 us, 133 TFLOP/s.  Parts switched off in turn: the loads
+// alone take 298 us (the tiles still read 2.5 GB from L2) and hide behind the
+// products, which alone take 635; of those the waits for the slowest warp of a
+// stage cost 76, the scores 224, the weights 69, the values 171 and the lists and
+// ends 95.  A token reads each of its pages from shared memory by itself (32 KB
+// for 8 query heads), so shared memory, not the tensor cores (257 us at the warp
+// instructions' full rate), is what the products run into.  128-row tensor core
 // tiles would multiply every token by every page of the tile: with pages chosen
 // alike they would win, with pages chosen by chance they do eight times the
 // work.
