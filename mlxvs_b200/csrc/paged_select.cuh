@@ -35,6 +35,7 @@ struct SelectParams {
 };
 
 constexpr int SELECT_WARPS = 8;
+constexpr int SELECT_WARP_PAGES = 512;  // selected by one warp
 constexpr int SELECT_CODES = 2 * 256;  // bytes of a token's query codes, at most
 
 // d += a b: 16 x 32 by 32 x 8 signed bytes, 32-bit sums.
@@ -188,8 +189,9 @@ __device__ __forceinline__ void select_pages(const uint32_t* keys, int held, int
 // keys -> bins, and for prompts the instructions of the selection.  Both want
 // many blocks per SM: fetching the codes a step ahead as well took 143
 // registers and made prompts of 5,229 tokens slower (97 -> 144 us).  Now those
-// take 57 us, 32 single tokens with up to 500 pages 14 us, and 7 with up to 3,900
-// pages (27 MB of codes) 20 us.
+// take 56 us (8 to start, 18 for the query codes, 14 for the scores, 16 for the
+// selection), 32 single tokens with up to 500 pages 11 us, and 7 with up to 3,900
+// pages (27 MB of codes) 21 us, of which 9 for the scores and 8 for the selection.
 //
 // SEG: 64-byte segments of a page's codes (dim up to 32 SEG).
 template <class T, int TT, int SEG>
@@ -261,15 +263,26 @@ __global__ void __launch_bounds__(SELECT_WARPS * 32, SEG == 8 ? 2 : 4) paged_sel
       const int c = (lane & (lanes - 1)) * 8, step = 32 / lanes;
       const bool mine = c < p.dim;
       const T* q = static_cast<const T*>(p.q) + t * p.q_token + (int64_t)h * p.group * p.q_head + c;
-      float top = 0.0f;
-      if (mine)
-#pragma unroll 4
-        for (int g = lane / lanes; g < p.group; g += step) {
-          const uint4 x = *reinterpret_cast<const uint4*>(q + g * p.q_head);
-          const T* e = reinterpret_cast<const T*>(&x);
+      // the first heads' values stay in registers between the two passes
+      constexpr int HELD = 4;
+      uint4 first[HELD];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(to_float(e[i])));
-        }
+      for (int u = 0; u < HELD; ++u) {
+        const int g = lane / lanes + u * step;
+        first[u] = mine && g < p.group ? *reinterpret_cast<const uint4*>(q + g * p.q_head)
+                                       : make_uint4(0, 0, 0, 0);
+      }
+      float top = 0.0f;
+      auto measure = [&](const uint4& x) {
+        const T* e = reinterpret_cast<const T*>(&x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(to_float(e[i])));
+      };
+#pragma unroll
+      for (int u = 0; u < HELD; ++u) measure(first[u]);
+      if (mine)
+        for (int g = lane / lanes + HELD * step; g < p.group; g += step)
+          measure(*reinterpret_cast<const uint4*>(q + g * p.q_head));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
       const float by = exp2_int(code_exponent(top));
@@ -278,20 +291,22 @@ __global__ void __launch_bounds__(SELECT_WARPS * 32, SEG == 8 ? 2 : 4) paged_sel
       float sum[8], size[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum[i] = size[i] = 0.0f;
-      if (mine)
-#pragma unroll 4
-        for (int g = lane / lanes; g < p.group; g += step) {
-          const uint4 x = *reinterpret_cast<const uint4*>(q + g * p.q_head);
-          const T* e = reinterpret_cast<const T*>(&x);
+      auto add = [&](const uint4& x) {
+        const T* e = reinterpret_cast<const T*>(&x);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float y = to_float(e[i]) * by;
-            // 1.5 * 2^23 added and taken off: rounded to nearest even
-            const float r = fmaxf(-127.0f, fminf(127.0f, y)) + 12582912.0f - 12582912.0f;
-            const float z = y == y ? r : 0.0f;
-            sum[i] += z, size[i] += fabsf(z);
-          }
+        for (int i = 0; i < 8; ++i) {
+          const float y = to_float(e[i]) * by;
+          // 1.5 * 2^23 added and taken off: rounded to nearest even
+          const float r = fmaxf(-127.0f, fminf(127.0f, y)) + 12582912.0f - 12582912.0f;
+          const float z = y == y ? r : 0.0f;
+          sum[i] += z, size[i] += fabsf(z);
         }
+      };
+#pragma unroll
+      for (int u = 0; u < HELD; ++u) add(first[u]);
+      if (mine)
+        for (int g = lane / lanes + HELD * step; g < p.group; g += step)
+          add(*reinterpret_cast<const uint4*>(q + g * p.q_head));
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         for (int o = lanes; o < 32; o <<= 1) {
@@ -384,8 +399,14 @@ __global__ void __launch_bounds__(SELECT_WARPS * 32, SEG == 8 ? 2 : 4) paged_sel
     __syncthreads();
   if (rank != 0) return;
   if (TT == 1) {
-    select_pages<SELECT_WARPS>(keys, __shfl_sync(~0u, my_held, 0), p.n,
-                               p.out + (t0 * p.heads + h) * p.n, hist[0], counts);
+    // few pages: one warp is quicker than a block's barriers (32 tokens with up
+    // to 500 pages 12.2 -> 11.3 us; up to 2048 pages it makes no difference)
+    const int mine = __shfl_sync(~0u, my_held, 0);
+    int32_t* out = p.out + (t0 * p.heads + h) * p.n;
+    if (mine > SELECT_WARP_PAGES)
+      select_pages<SELECT_WARPS>(keys, mine, p.n, out, hist[0], counts);
+    else if (warp == 0)
+      select_pages<1>(keys, mine, p.n, out, hist[0], nullptr);
   } else if (warp < TT && t0 + warp < p.tokens) {
     select_pages<1>(keys + (int64_t)warp * p.width, __shfl_sync(~0u, my_held, warp), p.n,
                     p.out + ((t0 + warp) * p.heads + h) * p.n, hist[warp], nullptr);
