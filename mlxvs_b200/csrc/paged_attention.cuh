@@ -158,13 +158,16 @@ struct AttentionShape {
   static constexpr int PITCH = DP * (int)sizeof(C);  // bytes of a row in shared memory
   static constexpr int KT = PITCH <= 128 ? 32 : 16;  // keys of a warp's step
   static constexpr int STEP = 2 * KT * PITCH;        // bytes of a warp's step
-  static constexpr int WARPS = 4;
-  // Blocks per SM, as registers allow, and the ring that shared memory leaves
-  // each: three blocks with rings of two steps against two with three took
+  // Warps, blocks per SM as registers allow, and the ring that shared memory
+  // leaves each: three blocks with rings of two steps against two with three took
   // 166 for 175 us on long 8-bit caches, and 20 for 23 us on short lists of pages
-  // (the products' latency counts there), the same on others.
-  static constexpr int BLOCKS = STEP > 8192 ? 1 : NT == 1 && DP <= 128 ? 3 : 2;
-  static constexpr int STAGES = STEP > 8192 ? 3 : (BLOCKS == 3 ? 2 : 3) * (8192 / STEP);
+  // (the products' latency counts there), the same on others.  Rows of 512 bytes:
+  // two blocks of three warps against one of four 140 for 182 us (8 requests up
+  // to 112,749 keys, 16 heads a key head).
+  static constexpr int WARPS = STEP > 8192 ? 3 : 4;
+  static constexpr int BLOCKS = STEP <= 8192 && NT == 1 && DP <= 128 ? 3 : 2;
+  static constexpr int STAGES =
+      STEP > 8192 ? 2 : (BLOCKS == 3 ? 2 : 3) * (8192 / STEP);
   static constexpr int KEYS = WARPS * KT;  // keys of a tile
   static constexpr int HEADS = 8 * NT;
   static constexpr int RING = WARPS * STAGES * STEP;
