@@ -545,7 +545,9 @@ MLXVS_C_API int mlxvs_profile_enable(int32_t on);
 
 /**
  * Total device time in ms and launch count of the recorded launches of one
- * kernel ("prep", "gemm_topk", "merge", "hamming_topk", "sumsq", "fill"), or
+ * kernel ("prep", "gemm_topk", "merge", "hamming_topk", "sumsq", "fill",
+ * "paged_tables", "paged_store", "paged_select", "paged_attention",
+ * "paged_attention_join", "paged_prompt"), or
  * of all of them when kernel is NULL.  Waits for the recorded events.
  */
 MLXVS_C_API int mlxvs_profile_read(const char* kernel, double* total_ms, int64_t* launches);

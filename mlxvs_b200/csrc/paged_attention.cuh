@@ -13,9 +13,9 @@
 // sum, weighted values) that a second kernel joins in the order of the keys.
 //
 // Measured, with the joining kernel: 64 requests of 0 to 5,000 keys (bf16, 8 key
-// heads of 4) 67 us, 5.7 TB/s; 200 requests of up to 16,000 keys (f16, 4 key heads
-// of 16) 404 us, 6.5 TB/s, the rate of a copy; 3 requests of up to 200,001 keys in
-// e4m3 (8 key heads of 8) 171 us, 5.4 TB/s, where the warps' conversions and the
+// heads of 4) 66 us, 5.7 TB/s; 200 requests of up to 16,000 keys (f16, 4 key heads
+// of 16) 395 us, 6.7 TB/s, the rate of a copy; 3 requests of up to 200,001 keys in
+// e4m3 (8 key heads of 8) 168 us, 5.5 TB/s, where the warps' conversions and the
 // short ring show.
 #pragma once
 
