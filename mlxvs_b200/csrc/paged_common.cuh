@@ -33,7 +33,7 @@ __device__ __forceinline__ float to_float(T x) {
   return static_cast<float>(x);
 }
 
-// x rounded to T: to nearest even, e4m3 saturated at 448 (NaN stays NaN).
+// x rounded to T, to nearest even.
 template <class T>
 __device__ __forceinline__ T from_float(float x);
 template <>
@@ -43,10 +43,6 @@ __device__ __forceinline__ __nv_bfloat16 from_float(float x) {
 template <>
 __device__ __forceinline__ __half from_float(float x) {
   return __float2half_rn(x);
-}
-template <>
-__device__ __forceinline__ __nv_fp8_e4m3 from_float(float x) {
-  return __nv_fp8_e4m3(x);
 }
 
 // The exponent e of an 8-bit code x * 2^e for values of at most `top` in
