@@ -438,9 +438,10 @@ MLXVS_C_API int mlxvs_paged_tables_device(
  * times the float32 reciprocals of the cache's scales, rounded to its type
  * (e4m3 saturates at 448); slots outside the cache are skipped.  Where the cache has codes and
  * scales, the bounds of every page that got a row are made anew over its rows
- * up to the last new one.  Slots must differ; a page's new rows come one
- * after another, as mlxvs_paged_tables_device gives them.  NaN keys do not
- * count in the bounds, infinite ones saturate.
+ * up to the last new one.  Slots must differ; a page's new rows are tokens in
+ * a row, one row on for each token, as mlxvs_paged_tables_device gives them.
+ * Any of those tokens may be skipped: its row keeps what it held.  NaN keys do
+ * not count in the bounds, infinite ones saturate.
  */
 MLXVS_C_API int mlxvs_paged_store_device(
     const mlxvs_paged_cache* cache,

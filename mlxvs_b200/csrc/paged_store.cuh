@@ -90,12 +90,18 @@ struct Range<__nv_bfloat16> {
   }
 };
 
-// One warp per key head and chunk of up to 32 tokens, LANES lanes per row (8
+// One warp per key head and chunk of up to 16 tokens, LANES lanes per row (8
 // channels each, so 16-byte loads), ROWS rows side by side.  First it copies
 // the chunk's rows; then, for each page whose last new row lies in the chunk,
 // it reads the page's rows (the new ones from the input, which other warps may
 // still be writing to the cache, the older ones from the cache) and makes its
 // bounds.  The second reading of new rows hits L2.
+//
+// A page's new rows are tokens in a row, one row on for each token; a skipped
+// token among them leaves its row as it was.  So row r of a page is new if token
+// te - re + r has its slot (te: the page's last token, re: its row), and a token
+// is its page's last unless the next token that is not skipped has its slot as
+// many rows on as it comes tokens later.
 //
 // Bound: the copies by HBM; single tokens by the latency of slot -> rows of
 // the page -> codes.  13,881 tokens of 8 heads of 128 into e4m3 take 23.7 us (86
@@ -117,14 +123,20 @@ __global__ void __launch_bounds__(STORE_WARPS * 32)
   C* values = static_cast<C*>(p.values) + h * p.value_head + d;
 
   // one token per lane: its page and row, and whether it is its page's last
+  const int64_t end = p.pages * P;  // of the slots
   int64_t slot = -1, page = -1;
   int row = 0;
-  bool last = false;
+  bool last = false, unsure = false;  // unsure: the next token is a skipped one
   if (lane < count) {
     slot = p.slots[t0 + lane];
-    if (slot >= 0 && slot < p.pages * P) {
+    if (slot >= 0 && slot < end) {
       page = slot / P, row = (int)(slot - page * P);
-      last = !(row + 1 < P && t0 + lane + 1 < p.tokens && p.slots[t0 + lane + 1] == slot + 1);
+      last = true;
+      if (row + 1 < P && t0 + lane + 1 < p.tokens) {
+        const int64_t next = p.slots[t0 + lane + 1];
+        last = next != slot + 1;
+        unsure = next < 0 || next >= end;
+      }
     }
   }
   constexpr int UNROLL = 4;
@@ -153,20 +165,42 @@ __global__ void __launch_bounds__(STORE_WARPS * 32)
   }
   if (p.codes == nullptr) return;
 
+  for (uint32_t some = __ballot_sync(~0u, unsure); some != 0; some &= some - 1) {
+    const int i = __ffs(some) - 1;
+    const int64_t t = t0 + i, s = __shfl_sync(~0u, slot, i);
+    const int reach = (int)min(P - 1 - __shfl_sync(~0u, row, i), p.tokens - 1 - t);
+    bool more = false;
+    for (int j0 = 2; j0 <= reach; j0 += 32) {
+      const int j = j0 + lane;
+      const int64_t later = j <= reach ? p.slots[t + j] : -1;
+      const uint32_t there = __ballot_sync(~0u, later >= 0 && later < end);
+      if (there != 0) {
+        more = __shfl_sync(~0u, later == s + j, __ffs(there) - 1);
+        break;
+      }
+    }
+    if (lane == i) last = !more;
+  }
   for (uint32_t ends = __ballot_sync(~0u, last); ends != 0; ends &= ends - 1) {
     const int e = __ffs(ends) - 1;
     const int64_t te = t0 + e;
     const int64_t pg = __shfl_sync(~0u, page, e), se = __shfl_sync(~0u, slot, e);
     const int re = __shfl_sync(~0u, row, e);
-    // the page's first new row: its new rows are the tokens te, te - 1, ...
+    // new rows without a gap, from the last one back: begin to re
     int begin = re;
+    bool gap = false;  // a skipped token lies before them
     while (begin > 0) {
       const int back = re - begin + 1 + lane;  // this lane's row is re - back
-      const bool fresh = back <= re && back <= te && p.slots[te - back] == se - back;
-      const uint32_t all = __ballot_sync(~0u, fresh);
+      const bool inside = back <= re && back <= te;
+      const int64_t s = inside ? p.slots[te - back] : 0;
+      const uint32_t all = __ballot_sync(~0u, inside && s == se - back);
+      const uint32_t skips = __ballot_sync(~0u, inside && (s < 0 || s >= end));
       const int run = all == ~0u ? 32 : __ffs(~all) - 1;
       begin -= run;
-      if (run < 32) break;
+      if (run < 32) {
+        gap = skips >> run & 1;
+        break;
+      }
     }
     // old rows as they are stored (e4m3 as the float16 it is exactly), new ones
     // as they came
@@ -175,23 +209,33 @@ __global__ void __launch_bounds__(STORE_WARPS * 32)
     Range<T> new_range;
     if (mine) {
       const C* old = keys + pg * p.key_page;
-#pragma unroll 8
-      for (int r = sub; r < begin; r += ROWS) {
+      const T* fresh = k + (te - re) * p.k_token;  // of the page's row 0, were it new
+      auto take_old = [&](int r) {
         const Eight<C> x = *reinterpret_cast<const Eight<C>*>(old + r * p.key_row);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           old_range.take(i, sizeof(C) == 1
                                 ? widen_e4m3(reinterpret_cast<const uint16_t*>(&x)[i])
                                 : reinterpret_cast<const uint32_t*>(&x)[i]);
-      }
-      const T* fresh = k + (te - re) * p.k_token;  // of the page's row 0, were it new
-#pragma unroll 8
-      for (int r = begin + sub; r <= re; r += ROWS) {
+      };
+      auto take_new = [&](int r) {
         const Eight<T> x = *reinterpret_cast<const Eight<T>*>(fresh + r * p.k_token);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           new_range.take(i, reinterpret_cast<const uint32_t*>(&x)[i]);
+      };
+      if (!gap) {
+#pragma unroll 8
+        for (int r = sub; r < begin; r += ROWS) take_old(r);
+      } else {
+        for (int r = sub; r < begin; r += ROWS) {
+          const int64_t t = te - re + r;
+          if (t >= 0 && p.slots[t] == se - re + r) take_new(r);
+          else take_old(r);
+        }
       }
+#pragma unroll 8
+      for (int r = begin + sub; r <= re; r += ROWS) take_new(r);
     }
     float lo[8], hi[8];
     {

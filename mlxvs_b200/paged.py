@@ -193,10 +193,13 @@ def paged_tables(past, fresh, table, free_pages, page_size, num_tokens, *, strea
 def paged_store(k, v, slots, keys, values, codes=None, scales=None, *, k_scale=1.0, v_scale=1.0,
                 stream=None):
     """Writes the rows k, v [tokens, key heads, dim] to their slots (int64, as
-    paged_tables gives them; negative ones are skipped) of the cache, times the
+    paged_tables gives them; those outside the cache are skipped), times the
     float32 reciprocals of k_scale / v_scale, rounded to the cache's type,
     which is k's or float8_e4m3fn (saturating).  With codes and scales, the bounds of every
-    page that got a row are renewed."""
+    page that got a row are renewed, over its rows up to the last new one.
+
+    Slots must differ, and a page's new rows be tokens in a row, one row on for
+    each token; any of them may be skipped, which leaves its row as it was."""
     op = "mlxvs::paged_store"
     lib = _load()
     ks = _rows(k, op, "k", _K_DIMS)

@@ -1,0 +1,65 @@
+"""GPU tests of the paged cache's operators at the edges of their inputs:
+skipped tokens, odd values in what the device reads, several host threads.
+Whole numbers are equal; tolerances stand at the tests that have one."""
+
+import numpy as np
+import pytest
+
+import mlxvs_b200 as mv
+from oracle import paged as O
+from tests.test_gpu_paged import dtype, make_cache, make_table, on_gpu, torch_, wide
+
+pytestmark = pytest.mark.gpu
+
+
+# past, fresh, page, heads, dim, type, cache, share of skipped tokens
+GAPS = [
+    ([3, 64, 100], [70, 64, 29], 64, 2, 128, "bfloat16", "float8_e4m3fn", 0.1),
+    ([0, 30, 7], [100, 3, 0], 24, 3, 80, "float16", "float16", 0.5),
+    ([1000, 1], [30, 1030], 1024, 1, 16, "bfloat16", "bfloat16", 0.97),
+    ([5] * 70, [2] * 70, 48, 8, 128, "bfloat16", "bfloat16", 0.5),
+    # chunks of several tokens: 16 at most from 148 * 16 * 16 / 8 tokens on
+    ([17, 0, 5], [3000, 2000, 1900], 128, 8, 64, "float16", "float8_e4m3fn", 0.05),
+    ([0], [2500], 1, 8, 64, "float16", "float16", 0.3),
+]
+
+
+@pytest.mark.parametrize("past,fresh,page,heads,dim,kind,cache,share", GAPS)
+def test_store_with_skipped_tokens(past, fresh, page, heads, dim, kind, cache, share):
+    """Any of a page's new tokens may be skipped: the page's bounds cover its
+    rows up to the last written one, whatever blocks write them."""
+    torch = torch_()
+    rng = np.random.default_rng(page + dim)
+    held = [a + b for a, b in zip(past, fresh)]
+    pages = sum(-(-x // page) for x in held) + 2
+    start = make_cache(rng, pages, page, heads, dim, cache)
+    table = make_table(rng, held, page, pages)
+    slots = np.concatenate([[table[r, i // page] * page + i % page for i in range(a, a + b)]
+                            for r, (a, b) in enumerate(zip(past, fresh))]).astype(int)
+    slots = np.concatenate([slots, np.full(100, -1)])  # padding
+    for _ in range(3):
+        at = slots.copy()
+        skipped = rng.random(len(at)) < share
+        at[skipped] = rng.choice([-1, pages * page, pages * page + 77], skipped.sum())
+        k = torch.from_numpy(3 * rng.standard_normal((len(at), heads, dim))).cuda().to(dtype(kind))
+        live = (at >= 0) & (at < pages * page)
+        where = torch.from_numpy(at[live]).cuda()
+        want = start[0].clone()
+        want[where // page, where % page] = k[torch.from_numpy(live).cuda()].to(want.dtype)
+        last = {}
+        for s in at[live]:
+            last[s // page] = max(last.get(s // page, 0), s % page)
+        rows = wide(want)
+        codes = np.full((pages, heads, 2, dim), 77)
+        scales = np.full((pages, heads), -1.0)
+        for p, row in last.items():
+            for h in range(heads):
+                codes[p, h], scales[p, h] = O.page_bounds(rows[p, :row + 1, h])
+        codes, scales = on_gpu(codes, "int8"), on_gpu(scales, "float32")
+        where = on_gpu(at, "int64")
+        for _ in range(20):
+            keys, values = start[0].clone(), start[1].clone()
+            got = torch.full_like(codes, 77), torch.full_like(scales, -1.0)
+            mv.paged_store(k, k, where, keys, values, *got)
+            assert torch.equal(keys.view(torch.uint8), want.view(torch.uint8))
+            assert torch.equal(got[0], codes) and torch.equal(got[1], scales)
