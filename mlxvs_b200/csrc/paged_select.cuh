@@ -55,8 +55,8 @@ __device__ __forceinline__ void select_sync() {
   else __syncthreads();
 }
 
-// The n pages of the best keys (0: no page, ~0: a forced one) of held pages,
-// ascending, by WARPS warps.  The range of the keys is cut into 256 bins, then
+// The n pages of the best keys (0: no page, 1: a score that is NaN, ~0: a forced
+// page) of held pages, ascending, by WARPS warps.  The range of the keys is cut into 256 bins, then
 // the bin that holds the n-th key again, until its count is taken whole or it
 // is a single key (whose first pages are taken): two rounds for most rows, four
 // at most.
@@ -91,7 +91,7 @@ __device__ __forceinline__ void select_pages(const uint32_t* keys, int held, int
   }
   // taken: keys above `limit`, and the first `equals` of those equal to it
   uint32_t limit = 0, equals = 0, need = (uint32_t)n - min((uint32_t)n, forced);
-  if (valid > need && need == 0) limit = FORCED, equals = n;
+  if (need == 0) limit = FORCED, equals = n;
   while (valid > need && need > 0) {
     const int bits = 32 - __clz(hi - lo), shift = max(bits - 8, 0);
     for (int i = tid; i < 256; i += THREADS) bins[i] = 0;
@@ -375,11 +375,15 @@ __global__ void __launch_bounds__(SELECT_WARPS * 32, SEG == 8 ? 2 : 4) paged_sel
         const int page = i < 2 ? b0 : b1;
         if (w >= TT || row_w[i & 1] != row || page >= held_w[i & 1]) continue;
         uint32_t key = 0;
-        if ((i < 2 ? id.x : id.y) >= 0)
-          // + 0.0f: a zero score has one form
-          key = page < p.first || page >= held_w[i & 1] - p.last
-                    ? 0xFFFFFFFFu
-                    : order_bits((float)dot[i] * (i < 2 ? scale0 : scale1) + 0.0f);
+        if ((i < 2 ? id.x : id.y) >= 0) {
+          // + 0.0f: a zero score has one form.  A NaN score (a scale that is not a
+          // number, or an infinite one times zero) comes after all others: by its
+          // bits it would be a forced page, of which there may be no more than n.
+          const float score = (float)dot[i] * (i < 2 ? scale0 : scale1) + 0.0f;
+          key = page < p.first || page >= held_w[i & 1] - p.last ? 0xFFFFFFFFu
+                : score == score                                 ? order_bits(score)
+                                                                 : 1u;
+        }
         const uint32_t at = (uint32_t)(w * p.width + page);
         if (cluster > 1)
           asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(first_keys + 4 * at), "r"(key)

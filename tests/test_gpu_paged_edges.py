@@ -63,3 +63,39 @@ def test_store_with_skipped_tokens(past, fresh, page, heads, dim, kind, cache, s
             mv.paged_store(k, k, where, keys, values, *got)
             assert torch.equal(keys.view(torch.uint8), want.view(torch.uint8))
             assert torch.equal(got[0], codes) and torch.equal(got[1], scales)
+
+
+def select_case(rng, count, widths, tokens, heads=2, group=4, dim=64):
+    """Codes of `count` pages, a table with a row per width and tokens that see
+    all of their request's pages (of 16 rows)."""
+    codes = np.sort(rng.integers(-127, 128, (count, heads, 2, dim)), 2)
+    table = np.full((len(widths), max(widths)), -1)
+    for r, w in enumerate(widths):
+        table[r, :w] = rng.integers(0, count, w)
+    requests = rng.integers(0, len(widths), tokens)
+    lengths = np.array(widths)[requests] * 16 - rng.integers(0, 16, tokens)
+    q = torch_().from_numpy(rng.standard_normal((tokens, heads * group, dim))).cuda().half()
+    return codes, table, requests, lengths, q
+
+
+@pytest.mark.parametrize("share", [1.0, 0.6])
+@pytest.mark.parametrize("widths,tokens", [([40], 1), ([700, 60], 2), ([100, 30, 9], 50)])
+def test_select_of_scores_that_are_not_numbers(widths, tokens, share):
+    """Scales that are NaN, or infinite where the codes are zero: NaN scores come
+    last, lists keep to their n entries."""
+    rng = np.random.default_rng(20)
+    n = 5
+    codes, table, requests, lengths, q = select_case(rng, 300, widths, tokens)
+    codes[::7] = 0  # infinite scales times zero
+    scales = 2.0 ** rng.integers(-3, 3, (300, 2))
+    odd = rng.random(scales.shape) < share
+    scales[odd] = np.nan
+    scales[::7][odd[::7]] = np.inf
+    for first, last in ((1, 1), (0, 0), (5, 0), (2, 3)):
+        with np.errstate(all="ignore"):
+            want = O.paged_select(wide(q), codes, scales, table, lengths, 16, n, requests, first,
+                                  last)
+        got = mv.paged_select(q, on_gpu(codes, "int8"), on_gpu(scales, "float32"), on_gpu(table),
+                              on_gpu(lengths), 16, n, requests=on_gpu(requests), first=first,
+                              last=last)
+        assert np.array_equal(got.cpu().numpy(), want)
