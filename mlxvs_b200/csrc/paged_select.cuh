@@ -124,7 +124,9 @@ __device__ __forceinline__ void select_pages(const uint32_t* keys, int held, int
     bin = __shfl_sync(~0u, bin, owner), in_bin = __shfl_sync(~0u, in_bin, owner);
     need -= __shfl_sync(~0u, above, owner);
     lo += bin << shift;
-    hi = min(hi, lo + ((1u << shift) - 1));
+    // the bin's end, which may lie past the largest 32-bit number (scores of over 1.7e38)
+    const uint32_t width = (1u << shift) - 1;
+    if (hi - lo > width) hi = lo + width;
     if (in_bin == need) {
       limit = lo - 1;  // lo > 0: keys of pages are
       break;

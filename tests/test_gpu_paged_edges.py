@@ -99,3 +99,24 @@ def test_select_of_scores_that_are_not_numbers(widths, tokens, share):
                               on_gpu(lengths), 16, n, requests=on_gpu(requests), first=first,
                               last=last)
         assert np.array_equal(got.cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("widths,tokens", [([40], 1), ([700, 60], 2), ([100, 30, 9], 50)])
+def test_select_of_infinite_scores(widths, tokens):
+    """Infinite scores of both signs beside finite ones: the largest order bits
+    that there are."""
+    rng = np.random.default_rng(21)
+    codes, table, requests, lengths, q = select_case(rng, 300, widths, tokens)
+    codes[codes == 0] = 1
+    for share in (0.02, 0.5):
+        scales = 2.0 ** rng.integers(-100, 101, (300, 2))
+        odd = rng.random(scales.shape) < share
+        scales[odd] = rng.choice([np.inf, -np.inf], odd.sum())
+        for n in (1, 3, 8):
+            with np.errstate(all="ignore"):  # a few dot products are 0: NaN
+                want = O.paged_select(wide(q), codes, scales, table, lengths, 16, n, requests, 0,
+                                      0)
+            got = mv.paged_select(q, on_gpu(codes, "int8"), on_gpu(scales, "float32"),
+                                  on_gpu(table), on_gpu(lengths), 16, n,
+                                  requests=on_gpu(requests), first=0, last=0)
+            assert np.array_equal(got.cpu().numpy(), want)
