@@ -309,7 +309,7 @@ void paged_select(const mlxvs_paged_cache& c, const mlxvs_paged_queries& q, int 
   check_codes(op, c);
   check_queries(op, c, q);
   REQUIRE(n >= 1 && n <= MAX_SELECTED, "n must be in [1, 256].");
-  REQUIRE(first >= 0 && last >= 0 && first + last <= n,
+  REQUIRE(first >= 0 && last >= 0 && first <= n && last <= n - first,
           "first and last must be at least 0 and together at most n.");
   REQUIRE(q.tokens == 0 || pages != nullptr, "pages must not be NULL.");
   DeviceInfo& dev = device_info();
