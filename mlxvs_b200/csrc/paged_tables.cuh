@@ -4,6 +4,8 @@
 // b0 = ceil(past / P) so far and needs b1 = min(ceil((past + fresh) / P), W);
 // the free list's pages are handed out in request order, so page b0 + i of a
 // request is free[off + i] with off the exclusive prefix sum of b1 - b0.
+// Lengths or sums of 2^31 and more (which the caller rules out) give wrong tokens,
+// but no place outside the table or the free list is read or written for them.
 // Everything a token needs follows from (past, first token, off) of its
 // request, so blocks share nothing: each one scans all requests (8 bytes a
 // request, from L2) and keeps those that its own range of tokens meets.  One
@@ -87,7 +89,8 @@ __global__ void __launch_bounds__(TABLES_THREADS) paged_tables_kernel(const Tabl
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
       b0[i] = (int)p.page.div((uint32_t)past[i] + P - 1);
-      const int b1 = min((int)p.page.div((uint32_t)past[i] + fresh[i] + P - 1), (int)p.width);
+      const uint32_t end = min((uint32_t)past[i] + (uint32_t)fresh[i], (uint32_t)INT32_MAX);
+      const int b1 = (int)min((int64_t)p.page.div(end + P - 1), p.width);
       need[i] = max(b1 - b0[i], 0);
       mine.x += fresh[i], mine.y += need[i];
     }
@@ -97,22 +100,24 @@ __global__ void __launch_bounds__(TABLES_THREADS) paged_tables_kernel(const Tabl
     const bool range_meets = base.x < t1 && base.x + total.x > t0;
     base.x += total.x, base.y += total.y;
     int at = count;
+    uint32_t kept = 0;  // a bit for each request of the thread
     if (range_meets) {
       // some request of these may meet the block's tokens: keep those, in order
-      int meets = 0, first = start;
+      int first = start;
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
-        meets += fresh[i] > 0 && first < t1 && first + fresh[i] > t0;
+        kept |= (uint32_t)(fresh[i] > 0 && first < t1 && first + fresh[i] > t0) << i;
         first += fresh[i];
       }
+      const int meets = __popc(kept);
       sum = block_scan3(make_int3(meets, 0, 0), warp_sums, &total);
       at += sum.x - meets;
-      count += total.x;
+      count = min(count + total.x, TABLES_TOKENS);
     }
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
       const int64_t r = r0 + threadIdx.x * ITEMS + i;
-      if (range_meets && fresh[i] > 0 && start < t1 && start + fresh[i] > t0)
+      if ((kept >> i & 1) && at < TABLES_TOKENS)
         met[at++] = make_int4(start, past[i], (int)r, off - b0[i]);
       if (writer && r < p.requests) {
         p.starts[r] = start;
@@ -120,9 +125,8 @@ __global__ void __launch_bounds__(TABLES_THREADS) paged_tables_kernel(const Tabl
           // tokens that get no slot: past the table's width, past the end of
           // the free list, or in a begun page that the table does not hold
           const int64_t avail = max((int64_t)0, min((int64_t)need[i], p.num_free - off));
-          const int end = past[i] + fresh[i];
-          const int64_t held =
-              min(min((int64_t)end, (b0[i] + avail) * P), (int64_t)width_tokens);
+          const int64_t end = (int64_t)past[i] + fresh[i];
+          const int64_t held = min(min(end, (b0[i] + avail) * P), (int64_t)width_tokens);
           int64_t lost = end - max(held, (int64_t)past[i]);
           const int begun = past[i] % P == 0 ? 0 : min(fresh[i], P - past[i] % P);
           if (begun > 0 && past[i] < width_tokens &&
@@ -157,15 +161,15 @@ __global__ void __launch_bounds__(TABLES_THREADS) paged_tables_kernel(const Tabl
       row[u] = -1, length[u] = 0, page[u] = -1;
       if (t < t1 && t < base.x && lo > 0) {
         const int4 m = met[lo - 1];
-        const int pos = m.y + (t - m.x);
-        row[u] = m.z, length[u] = pos + 1;
-        if (pos < width_tokens) {
+        const uint32_t pos = (uint32_t)m.y + (uint32_t)t - (uint32_t)m.x;
+        row[u] = m.z, length[u] = (int)min(pos, (uint32_t)INT32_MAX - 1) + 1;
+        if (pos < (uint32_t)width_tokens) {
           const int b = (int)p.page.div(pos);
-          in[u] = pos - b * P;
+          in[u] = (int)pos - b * P;
           const bool fresh = b * P >= m.y;  // handed out in this step
           const int64_t place = (int64_t)m.z * p.width + b, listed = (int64_t)m.w + b;
           if (!fresh) page[u] = p.table[place];
-          else if (listed < p.num_free) page[u] = p.free_pages[listed];
+          else if (listed >= 0 && listed < p.num_free) page[u] = p.free_pages[listed];
           entry[u] = fresh && in[u] == 0 ? place : -1;
         } else {
           in[u] = 0, entry[u] = -1;

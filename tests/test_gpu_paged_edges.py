@@ -120,3 +120,38 @@ def test_select_of_infinite_scores(widths, tokens):
                                   on_gpu(table), on_gpu(lengths), 16, n,
                                   requests=on_gpu(requests), first=0, last=0)
             assert np.array_equal(got.cpu().numpy(), want)
+
+
+def test_tables_of_impossible_lengths():
+    """Lengths and sums past 2^31 (which the caller rules out): what lies about
+    the table stays, slots are in the free pages or -1, requests before the
+    impossible one are right."""
+    torch = torch_()
+    rng = np.random.default_rng(22)
+    top = 2 ** 31 - 1
+    free = np.arange(50, 150)
+
+    def run(past, fresh, page, width, tokens):
+        room = torch.full((3, len(past), width), -9, dtype=torch.int32, device="cuda")
+        room[1] = -1
+        got = mv.paged_tables(on_gpu(past), on_gpu(fresh), room[1], on_gpu(free), page, tokens)
+        mv.synchronize()
+        assert (room[0] == -9).all() and (room[2] == -9).all()
+        slots = got.slots.cpu().numpy()
+        assert ((slots == -1) | ((slots >= 50 * page) & (slots < 150 * page))).all()
+        return got, room[1]
+
+    for page in (1, 16, 1000):
+        for wild in ((top, 1), (top, 9), (top - 1, 3)):
+            got, table = run([0, wild[0], 0], [3, wild[1], 2], page, 4, 40)
+            want = O.paged_tables([0], [3], np.full((1, 4), -1), free, page, 3)
+            assert np.array_equal(table[:1].cpu().numpy(), want[0])
+            assert np.array_equal(got.slots[:3].cpu().numpy(), want[4])
+            assert got.requests[:3].tolist() == [0] * 3 and got.lengths[:3].tolist() == [1, 2, 3]
+    for _ in range(20):
+        for requests in (3, 300, 6000):
+            past = rng.integers(0, top, requests, endpoint=True)
+            past[rng.random(requests) < 0.5] //= 2 ** 28
+            fresh = rng.integers(-2 ** 31, top, requests, endpoint=True)
+            run(past, fresh, int(rng.integers(1, 70)), int(rng.integers(1, 9)),
+                int(rng.integers(1, 9000)))
