@@ -103,12 +103,16 @@ void check_queries(const char* op, const mlxvs_paged_cache& c,
           "q must be 16-byte aligned, with strides of multiples of 16 bytes.");
 }
 
-// More than 48 KB of shared memory, with the kernel's static arrays (at most 16
-// KB here), has to be asked for.
+// What the kernels' static arrays may take of a block's shared memory.
+constexpr int STATIC_SMEM = 16384;
+
+// More than 48 KB of shared memory, static arrays among it, has to be asked for.
+// The limit belongs to the kernel, not to the call, and other threads launch it
+// too: `most` is one number for all of a kernel's calls.
 template <class K>
-void allow_smem(K* kernel, size_t bytes) {
+void allow_smem(K* kernel, size_t bytes, size_t most) {
   if (bytes > 32 * 1024)
-    CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
 }
 
 // The attention kernel on every SM and, when it may have cut rows, the kernel
@@ -118,7 +122,7 @@ void launch_attention(AttentionParams p, DeviceInfo& dev, Scratch& scratch, cuda
   using S = AttentionShape<T, C, DP, NT>;
   auto* kernel = p.selected ? paged_attention_kernel<T, C, DP, NT, true>
                             : paged_attention_kernel<T, C, DP, NT, false>;
-  allow_smem(kernel, S::SMEM);
+  allow_smem(kernel, S::SMEM, S::SMEM);
   // Rows of few tiles are not cut: a block each, and no second kernel.  Longest
   // possible rows of 8 tiles: two requests of up to 300 keys 8.1 -> 6.0 us in a
   // graph (and one launch less on the host), 415 tokens with 9 pages of 24 and
@@ -215,7 +219,7 @@ void launch_prompt(const AttentionParams& p, DeviceInfo& dev, cudaStream_t s) {
   const CUtensorMap values =
       cache_map<C>(p.values, p, p.value_head, p.value_row, p.value_page, S::BOX);
   auto* kernel = paged_prompt_kernel<T, C, DP>;
-  allow_smem(kernel, S::SMEM);
+  allow_smem(kernel, S::SMEM, S::SMEM);
   const dim3 grid((unsigned)((p.tokens + pp.tile - 1) / pp.tile),
                   p.heads * ((p.group + 15) / 16));
   ProfScope prof("paged_prompt", s);
@@ -314,7 +318,7 @@ void paged_select(const mlxvs_paged_cache& c, const mlxvs_paged_queries& q, int 
   REQUIRE(q.tokens == 0 || pages != nullptr, "pages must not be NULL.");
   DeviceInfo& dev = device_info();
   // keys of one token and the static arrays must fit a block's shared memory
-  const int64_t room = (dev.max_smem - 16384) / 4;
+  const int64_t room = (dev.max_smem - STATIC_SMEM) / 4;
   REQUIRE(q.width <= room,
           "the table must have at most " + std::to_string(room) + " pages a request.");
   if (q.tokens == 0) return;
@@ -344,7 +348,7 @@ void paged_select(const mlxvs_paged_cache& c, const mlxvs_paged_queries& q, int 
                    : tiles        ? paged_select_kernel<T, 8, 8>
                                   : paged_select_kernel<T, 1, 8>;
     const size_t smem = (size_t)(tiles ? 8 : 1) * q.width * 4;
-    allow_smem(kernel, smem);
+    allow_smem(kernel, smem, dev.max_smem - STATIC_SMEM);
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3((unsigned)(units * cluster), c.heads);
     config.blockDim = dim3(SELECT_WARPS * 32);

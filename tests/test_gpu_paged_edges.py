@@ -155,3 +155,51 @@ def test_tables_of_impossible_lengths():
             fresh = rng.integers(-2 ** 31, top, requests, endpoint=True)
             run(past, fresh, int(rng.integers(1, 70)), int(rng.integers(1, 9)),
                 int(rng.integers(1, 9000)))
+
+
+def test_select_from_several_threads():
+    """Calls with tables of different widths from several host threads: their
+    kernels' shared memory differs, each launch is its call's own."""
+    import threading
+
+    from mlxvs_b200 import paged
+
+    torch = torch_()
+    lib = mv._load()
+    rng = np.random.default_rng(23)
+    dim, n = 64, 4
+    codes = on_gpu(np.sort(rng.integers(-127, 128, (50, 1, 2, dim)), 2), "int8")
+    scales = torch.ones(50, 1, device="cuda")
+    q = torch.randn(16, 1, dim, device="cuda").half()
+    cache = paged._CACHE.pack(0, 0, 0, 0, 0, 0, 0, 0, 50, codes.data_ptr(), scales.data_ptr(), 16,
+                              1, dim, 0, 1.0, 1.0)
+    requests, lengths = on_gpu([0] * 16), on_gpu([40 * 16] * 16)
+    calls = []
+    for width in (1200, 6000):  # 38 and 192 KB for tiles of 8 tokens
+        table = on_gpu(rng.integers(0, 50, (1, width)))
+        want = mv.paged_select(q, codes, scales, table, lengths, 16, n, requests=requests)
+        queries, _, _ = paged._queries(q, table, lengths, requests, "test")
+        calls.append((table, queries, want))
+    failed = []
+
+    def work(queries, want):
+        stream = torch.cuda.Stream()
+        out = torch.zeros_like(want)
+        stream.wait_stream(torch.cuda.current_stream())
+        args = (cache, queries, n, 1, 1, out.data_ptr(), stream.cuda_stream)
+        run = lib.mlxvs_paged_select_device
+        for _ in range(20000):
+            if run(*args):
+                failed.append(lib.mlxvs_last_error())
+                break
+        stream.synchronize()
+        if not torch.equal(out, want):
+            failed.append("another result")
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=calls[i % 2][1:]) for i in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
