@@ -85,7 +85,6 @@ __device__ __forceinline__ void prompt_keys(float (&o)[DP / 16][NT][4], float (&
                                             const float (*factor)[8]) {
   using S = PromptShape<T, C, DP>;
   using M = typename std::conditional<S::EIGHT, __half, T>::type;
-  constexpr bool TWO_TERMS = !S::EIGHT || std::is_same<T, __half>::value;
   const int lane = threadIdx.x & 31;
   auto chunk_at = [](int r, int c) -> uint32_t {
     constexpr int PER = S::BOX / 16;
@@ -186,10 +185,8 @@ __device__ __forceinline__ void prompt_keys(float (&o)[DP / 16][NT][4], float (&
           l[nt][0] += w0, l[nt][1] += w1;
           const uint32_t both = pack2<M>(w0, w1);
           b[mt][nt][u] = transpose8x8(both);
-          if (TWO_TERMS) {
-            const float2 r = unpack2<M>(both);
-            rest[mt][nt][u] = transpose8x8(pack2<M>(w0 - r.x, w1 - r.y));
-          }
+          const float2 r = unpack2<M>(both);
+          rest[mt][nt][u] = transpose8x8(pack2<M>(w0 - r.x, w1 - r.y));
         }
     }
   // ---- O^T += V^T P^T
@@ -216,7 +213,7 @@ __device__ __forceinline__ void prompt_keys(float (&o)[DP / 16][NT][4], float (&
             if (decltype(masked)::value)
               x[0] &= see[nt][0], x[1] &= see[nt][0], x[2] &= see[nt][1], x[3] &= see[nt][1];
             mma16816<M>(o[s][nt], x, b[mt][nt][0], b[mt][nt][1]);
-            if (TWO_TERMS) mma16816<M>(o[s][nt], x, rest[mt][nt][0], rest[mt][nt][1]);
+            mma16816<M>(o[s][nt], x, rest[mt][nt][0], rest[mt][nt][1]);
           }
       };
       if (S::EIGHT) {

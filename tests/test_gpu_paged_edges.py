@@ -7,7 +7,7 @@ import pytest
 
 import mlxvs_b200 as mv
 from oracle import paged as O
-from tests.test_gpu_paged import dtype, make_cache, make_table, on_gpu, torch_, wide
+from tests.test_gpu_paged import UNIT, dtype, make_cache, make_table, on_gpu, torch_, wide
 
 pytestmark = pytest.mark.gpu
 
@@ -203,3 +203,61 @@ def test_select_from_several_threads():
     for t in threads:
         t.join()
     assert not failed, failed
+
+
+FORMS = [("bfloat16", "bfloat16"), ("float16", "float16"), ("bfloat16", "float8_e4m3fn"),
+         ("float16", "float8_e4m3fn")]
+
+
+def attend_alike(kind, cache, k0, v0, scale, prompt, group=8, page=64):
+    """Attention of like tokens over like requests, by the kernel of single
+    tokens or the prompts'.  k0: channel 0 of the keys, where the queries are 1
+    and all else is 0; v0 [keys, dim].  Returns out [.., dim] and lse [..]."""
+    torch = torch_()
+    heads, dim = 8, v0.shape[1]
+    pages = -(-len(k0) // page)
+    keys = torch.zeros(pages * page, heads, dim, device="cuda")
+    values = torch.zeros_like(keys)
+    keys[:len(k0), :, 0] = on_gpu(k0, "float32")[:, None]
+    values[:len(k0)] = on_gpu(v0, "float32")[:, None]
+    keys, values = (x.view(pages, page, heads, dim).to(dtype(cache)) for x in (keys, values))
+    tokens, rows = (600, 1) if prompt else (64, 64)
+    q = torch.zeros(tokens, heads * group, dim, dtype=dtype(kind), device="cuda")
+    q[..., 0] = 1
+    table = on_gpu(np.arange(pages)[None].repeat(rows, 0))
+    more = {}
+    if prompt:
+        more = dict(requests=on_gpu([0] * tokens),
+                    pages=on_gpu(np.arange(pages)).expand(tokens, heads, -1).contiguous())
+    out, lse = mv.paged_attention(q, keys, values, table, on_gpu([len(k0)] * tokens), scale=scale,
+                                  return_lse=True, **more)
+    return wide(out).reshape(-1, dim), wide(lse).reshape(-1)
+
+
+def exact_alike(k0, v0, scale):
+    """The same for one token, in 64 bits, and its weights."""
+    s = np.asarray(k0, float) * float(np.float32(scale))
+    p = np.exp(s - s.max())
+    with np.errstate(all="ignore"):
+        return p @ v0 / p.sum(), s.max() + np.log(p.sum()), p / p.sum()
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("kind,cache", FORMS)
+def test_weights_where_values_cancel(kind, cache, prompt):
+    """200 keys of weight 1 and value 1, 400 of weight 0.5 (1 + 0.9 2^-11) and
+    value -1: the sum is what a weight's rounding to 11 bits would leave.
+
+    The weights' two terms leave 2^-17 of them at most, the tensor cores' sums
+    of at most 600 / 16 steps 38 2^-23, exponentials and scores (one product)
+    less than 2^-20: 2^-16 in all, and the output's own rounding."""
+    weight = 0.5 * (1 + 0.9 * 2.0 ** -11)
+    rng = np.random.default_rng(24)
+    second = np.zeros(600)
+    second[rng.permutation(600)[:400]] = 1
+    v0 = np.repeat((1 - 2 * second)[:, None], 64, 1)
+    scale = -np.log(weight)
+    want, want_lse, _ = exact_alike(-second, v0, scale)
+    out, lse = attend_alike(kind, cache, -second, v0, scale, prompt)
+    assert (np.abs(out - want) <= UNIT[kind] * np.abs(want) + 2.0 ** -16).all()
+    assert (np.abs(lse - want_lse) <= 2.0 ** -20 * (1 + abs(want_lse))).all()
