@@ -19,6 +19,8 @@
 // short ring show.
 #pragma once
 
+#include <type_traits>
+
 #include "paged_common.cuh"
 
 namespace mlxvs_b200 {
@@ -149,6 +151,37 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// ------------------------------------------------------------------ softmax
+// Weights are 2^(s - m) with a reference m that follows the running maximum: it
+// is LIFT below the maximum when it is raised, and raised when a score passes it
+// by LIFT + 8.  So weights stay below 2^(LIFT + 8) and the largest one of a row is
+// at least 2^LIFT.  In float16 LIFT is 7: weights up to 2^15 of 65,504, and the
+// smallest steps, 2^-24, are 2^-31 of the largest weight, so that what many small
+// weights behind a large one lose stays below the output's rounding up to 2^20
+// keys.  bfloat16 has the exponents of float32.
+template <class M>
+struct Lift {
+  static constexpr float value = std::is_same<M, __half>::value ? 7.0f : 0.0f;
+};
+// Rounded so that the weights' bounds hold for scores of any size.
+template <class M>
+__device__ __forceinline__ float reference(float maximum) {
+  return __fadd_ru(maximum, -Lift<M>::value);
+}
+template <class M>
+__device__ __forceinline__ float raised_past(float m) {
+  return __fadd_rd(m, Lift<M>::value + 8.0f);
+}
+
+// sum += x with what the addition loses kept in `lost` (Kahan, 1965): a thread's
+// sum of weights has one term per key, too many for plain float32 sums behind a
+// large one.
+__device__ __forceinline__ void add_kept(float& sum, float& lost, float x) {
+  const float y = x - lost, t = sum + y;
+  lost = (t - sum) - y;
+  sum = t;
+}
+
 // ------------------------------------------------------------------ shapes
 // T: type of the queries, C: of the cache, DP: the head dimension padded to
 // 64, 128 or 256, NT: query heads in eights (8 or 16 at a time).
@@ -195,9 +228,9 @@ struct AttentionRow {
 // than tiled ones: rows may lie in pages of any size).  Scores and sums
 // are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that the 16-row side
 // of the tensor cores' tile holds keys or channels, never padding, and the
-// 8-column side the query heads.  The running maximum is raised only when a
-// score passes it by 2^8: the weights then stay below 2^8, far from overflow,
-// and the sums are rescaled a few times a row instead of every step.
+// 8-column side the query heads.  The weights' reference is raised only when a
+// score passes the maximum it was taken from by 8, so the sums are rescaled a few
+// times a row instead of every step.
 //
 // The weights are two 16-bit terms (value and remainder), since one would add a
 // rounding up to as large as the output's own, and more where values cancel; the
@@ -490,10 +523,10 @@ __global__ void __launch_bounds__(AttentionShape<T, C, DP, NT>::WARPS * 32,
     const int tile0 = (int)(x - row.start);
     const int tile1 = (int)min((int64_t)row.tiles, x1 - row.start);
     scale_queries();
-    float o[DP / 16][NT][4], m[NT][2], l[NT][2];
+    float o[DP / 16][NT][4], m[NT][2], l[NT][2], lost[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m[nt][0] = m[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.0f;
+      m[nt][0] = m[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = lost[nt][0] = lost[nt][1] = 0.0f;
 #pragma unroll
       for (int i = 0; i < DP / 16; ++i)
         o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.0f;
@@ -549,7 +582,7 @@ __global__ void __launch_bounds__(AttentionShape<T, C, DP, NT>::WARPS * 32,
           }
         }
       }
-      // ---- scores, masked; a raised maximum where one passes it by 2^8
+      // ---- scores, masked; a raised reference where one passes it by far
       bool raise = false;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
@@ -560,27 +593,31 @@ __global__ void __launch_bounds__(AttentionShape<T, C, DP, NT>::WARPS * 32,
             float& s = st[mt][nt][i];
             s *= factor[nt][i & 1];
             if (!((valid >> (mt * 16 + (i >> 1) * 8 + lane / 4)) & 1)) s = -INFINITY;
-            raise |= s > m[nt][i & 1] + 8.0f;
+            raise |= s > raised_past<M>(m[nt][i & 1]);
           }
       if (__any_sync(~0u, raise)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            float top = m[nt][i];
+            float top = -INFINITY;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
               top = fmaxf(top, fmaxf(st[mt][nt][i], st[mt][nt][i + 2]));
 #pragma unroll
             for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, w));
-            const float keep = m[nt][i] == -INFINITY ? 0.0f : exp2_approx(m[nt][i] - top);
-            m[nt][i] = top;
-            l[nt][i] *= keep;
+            const float to = fmaxf(m[nt][i], reference<M>(top));
+            const float keep = m[nt][i] == -INFINITY ? 0.0f : exp2_approx(m[nt][i] - to);
+            m[nt][i] = to;
+            l[nt][i] *= keep, lost[nt][i] *= keep;
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k) o[k][nt][i] *= keep, o[k][nt][i + 2] *= keep;
           }
       }
       // ---- weights, and O^T += V^T P^T
+      float more[NT][2];  // the tile's weights
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) more[nt][0] = more[nt][1] = 0.0f;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         uint32_t b[NT][2], rest[NT][2];
@@ -592,7 +629,7 @@ __global__ void __launch_bounds__(AttentionShape<T, C, DP, NT>::WARPS * 32,
           for (int u = 0; u < 2; ++u) {
             const float w0 = exp2_approx(st[mt][nt][2 * u] - m0);
             const float w1 = exp2_approx(st[mt][nt][2 * u + 1] - m1);
-            l[nt][0] += w0, l[nt][1] += w1;
+            more[nt][0] += w0, more[nt][1] += w1;
             const uint32_t both = pack2<M>(w0, w1);
             b[nt][u] = transpose8x8(both);
             const float2 r = unpack2<M>(both);
@@ -634,6 +671,10 @@ __global__ void __launch_bounds__(AttentionShape<T, C, DP, NT>::WARPS * 32,
           }
         }
       }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) add_kept(l[nt][i], lost[nt][i], more[nt][i]);
     }
     // ---- on to the next row, whose queries are fetched meanwhile
     const AttentionRow ended = row;

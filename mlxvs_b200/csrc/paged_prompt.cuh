@@ -80,7 +80,7 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, u
 // products -> weights -> products.
 template <class T, class C, int DP, int NT, int WHICH, int MT>
 __device__ __forceinline__ void prompt_keys(float (&o)[DP / 16][NT][4], float (&m)[NT][2],
-                                            float (&l)[NT][2], uint32_t keys, uint32_t values,
+                                            float (&l)[NT][2], float (&lost)[NT][2], uint32_t keys, uint32_t values,
                                             uint32_t queries, int first, const int (&limit)[NT],
                                             const float (*factor)[8]) {
   using S = PromptShape<T, C, DP>;
@@ -134,7 +134,7 @@ __device__ __forceinline__ void prompt_keys(float (&o)[DP / 16][NT][4], float (&
       }
     }
   }
-  // ---- scores, masked; the maximum is raised where one passes it by 2^8
+  // ---- scores, masked; the reference is raised where one passes it by far
   bool raise = false, partial = false;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
@@ -148,7 +148,7 @@ __device__ __forceinline__ void prompt_keys(float (&o)[DP / 16][NT][4], float (&
           float& x = st[mt][nt][i];
           x *= i & 1 ? f.y : f.x;
           if (mt * 16 + (i >> 1) * 8 + lane / 4 >= limit[nt]) x = -INFINITY;
-          raise |= x > m[nt][i & 1] + 8.0f;
+          raise |= x > raised_past<M>(m[nt][i & 1]);
         }
     }
   if (__any_sync(~0u, raise)) {
@@ -157,14 +157,15 @@ __device__ __forceinline__ void prompt_keys(float (&o)[DP / 16][NT][4], float (&
       if (WHICH >> nt & 1)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float top = m[nt][i];
+          float top = -INFINITY;
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) top = fmaxf(top, fmaxf(st[mt][nt][i], st[mt][nt][i + 2]));
 #pragma unroll
           for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, w));
-          const float keep = m[nt][i] == -INFINITY ? 0.0f : exp2_approx(m[nt][i] - top);
-          m[nt][i] = top;
-          l[nt][i] *= keep;
+          const float to = fmaxf(m[nt][i], reference<M>(top));
+          const float keep = m[nt][i] == -INFINITY ? 0.0f : exp2_approx(m[nt][i] - to);
+          m[nt][i] = to;
+          l[nt][i] *= keep, lost[nt][i] *= keep;
 #pragma unroll
           for (int k = 0; k < DP / 16; ++k) o[k][nt][i] *= keep, o[k][nt][i + 2] *= keep;
         }
@@ -176,18 +177,21 @@ __device__ __forceinline__ void prompt_keys(float (&o)[DP / 16][NT][4], float (&
     if (WHICH >> nt & 1) {
       const float m0 = m[nt][0] == -INFINITY ? 0.0f : m[nt][0];
       const float m1 = m[nt][1] == -INFINITY ? 0.0f : m[nt][1];
+      float more[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const float w0 = exp2_approx(st[mt][nt][2 * u] - m0);
           const float w1 = exp2_approx(st[mt][nt][2 * u + 1] - m1);
-          l[nt][0] += w0, l[nt][1] += w1;
+          more[0] += w0, more[1] += w1;
           const uint32_t both = pack2<M>(w0, w1);
           b[mt][nt][u] = transpose8x8(both);
           const float2 r = unpack2<M>(both);
           rest[mt][nt][u] = transpose8x8(pack2<M>(w0 - r.x, w1 - r.y));
         }
+      add_kept(l[nt][0], lost[nt][0], more[0]);
+      add_kept(l[nt][1], lost[nt][1], more[1]);
     }
   // ---- O^T += V^T P^T
   auto products = [&](auto masked) {
@@ -347,10 +351,10 @@ __global__ void __launch_bounds__((PromptShape<T, C, DP>::WARPS + 1) * 32, 1)
   const uint32_t ring_at = smem_address(ring), q_base = smem_address(q_mem);
   const int entries = S::SLOTS / pp.slots;  // page pieces of a stage
   uint32_t stage = 0, phase = 0;            // of the next stage, by both sides
-  float o[DP / 16][NT][4], m[NT][2], l[NT][2];
+  float o[DP / 16][NT][4], m[NT][2], l[NT][2], lost[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    m[nt][0] = m[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.0f;
+    m[nt][0] = m[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = lost[nt][0] = lost[nt][1] = 0.0f;
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i)
       o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.0f;
@@ -461,7 +465,7 @@ __global__ void __launch_bounds__((PromptShape<T, C, DP>::WARPS + 1) * 32, 1)
             auto step = [&](auto which, auto tiles) {
               constexpr int MT = decltype(tiles)::value;
               prompt_keys<T, C, DP, NT, decltype(which)::value, MT>(
-                  o, m, l, kat, vat, queries, slot + k, limit, factor);
+                  o, m, l, lost, kat, vat, queries, slot + k, limit, factor);
               k += 16 * MT;
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) limit[nt] -= 16 * MT;

@@ -261,3 +261,22 @@ def test_weights_where_values_cancel(kind, cache, prompt):
     out, lse = attend_alike(kind, cache, -second, v0, scale, prompt)
     assert (np.abs(out - want) <= UNIT[kind] * np.abs(want) + 2.0 ** -16).all()
     assert (np.abs(lse - want_lse) <= 2.0 ** -20 * (1 + abs(want_lse))).all()
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("kind,cache", FORMS)
+def test_many_small_weights_behind_a_large_one(kind, cache, prompt):
+    """One key of value 0 and 4,095 keys of weight 2^-25.5 behind it: the output
+    is the small ones' alone.
+
+    Float16 weights are multiples of 2^-24, 2^-7 times that of the largest one:
+    off by 2^-32 at most each, the sum of 4,095 by 4,095 2^-32 times the value
+    (1.1 %), beside what values that cancel are held to."""
+    k0 = np.r_[0.0, np.full(4095, -1.0)]
+    v0 = np.r_[0.0, np.full(4095, 256.0)][:, None].repeat(64, 1)
+    scale = 25.5 * np.log(2)
+    want, want_lse, _ = exact_alike(k0, v0, scale)
+    out, lse = attend_alike(kind, cache, k0, v0, scale, prompt, group=1)
+    tol = (UNIT[kind] + 2.0 ** -13) * want + 4095 * 2.0 ** -32 * 256
+    assert (np.abs(out - want) <= tol).all()
+    assert (np.abs(lse - want_lse) <= 2.0 ** -20 * (1 + abs(want_lse))).all()
