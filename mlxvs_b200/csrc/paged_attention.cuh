@@ -135,6 +135,28 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t x) {
   return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u));
 }
 
+// Two values cut to a magnitude that no sum of products with the weights'
+// remainders carries to infinity (float16: 65,504, its largest; bfloat16: 2^110,
+// whose remainders are at most 1/2).  A remainder may be 0 or negative, and
+// times an infinite value it would make a NaN of the infinity that the weight's
+// first term gives.  (A float16 weight below 2^-32 of the largest is zero and
+// still makes one, as a float32 weight that underflows does.)  Prompts of 5,229
+// tokens 738 -> 754 us, 200 requests of up to 16,000 keys 463 -> 471 us (calls).
+template <class T>
+__device__ __forceinline__ uint32_t finite2(uint32_t x);
+template <>
+__device__ __forceinline__ uint32_t finite2<__half>(uint32_t x) {
+  uint32_t r;  // the smaller magnitude, with the signs' product
+  asm("min.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x7BFF7BFFu));
+  return r;
+}
+template <>
+__device__ __forceinline__ uint32_t finite2<__nv_bfloat16>(uint32_t x) {
+  uint32_t r;
+  asm("min.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x76807680u));
+  return r;
+}
+
 // Two e4m3 (the low 16 bits of x) as two float16: exact.
 __device__ __forceinline__ uint32_t widen_e4m3(uint32_t x) {
   uint32_t r;
@@ -664,10 +686,11 @@ __global__ void __launch_bounds__(AttentionShape<T, C, DP, NT>::WARPS * 32,
             uint32_t a[4];
             load_matrices_t(a, vat + chunk_at(r, 2 * s + ((lane >> 3) & 1)));
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma16816<M>(o[s][nt], a, b[nt][0], b[nt][1]);
-              mma16816<M>(o[s][nt], a, rest[nt][0], rest[nt][1]);
-            }
+            for (int nt = 0; nt < NT; ++nt) mma16816<M>(o[s][nt], a, b[nt][0], b[nt][1]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[i] = finite2<M>(a[i]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16816<M>(o[s][nt], a, rest[nt][0], rest[nt][1]);
           }
         }
       }

@@ -209,16 +209,23 @@ __device__ __forceinline__ void prompt_keys(float (&o)[DP / 16][NT][4], float (&
           see[nt][u] =
               (key < limit[nt] ? 0xFFFFu : 0u) | (key + 1 < limit[nt] ? 0xFFFF0000u : 0u);
         }
-      auto multiply = [&](const uint32_t (&w)[4], int s) {
+      auto multiply = [&](uint32_t (&w)[4], int s) {
+        auto product = [&](const uint32_t (&weights)[NT][2]) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          if (WHICH >> nt & 1) {
-            uint32_t x[4] = {w[0], w[1], w[2], w[3]};
-            if (decltype(masked)::value)
-              x[0] &= see[nt][0], x[1] &= see[nt][0], x[2] &= see[nt][1], x[3] &= see[nt][1];
-            mma16816<M>(o[s][nt], x, b[mt][nt][0], b[mt][nt][1]);
-            mma16816<M>(o[s][nt], x, rest[mt][nt][0], rest[mt][nt][1]);
-          }
+          for (int nt = 0; nt < NT; ++nt)
+            if (WHICH >> nt & 1) {
+              uint32_t x[4] = {w[0], w[1], w[2], w[3]};
+              if (decltype(masked)::value)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] &= see[nt][i / 2];
+              mma16816<M>(o[s][nt], x, weights[nt][0], weights[nt][1]);
+            }
+        };
+        product(b[mt]);
+        if (!S::EIGHT)  // an 8-bit cache has no infinities
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = finite2<M>(w[i]);
+        product(rest[mt]);
       };
       if (S::EIGHT) {
         const int r = first + mt * 16 + (lane & 15);
@@ -230,8 +237,8 @@ __device__ __forceinline__ void prompt_keys(float (&o)[DP / 16][NT][4], float (&
           for (int u = 0; u < 2; ++u) {
             const uint32_t e0 = __byte_perm(a[2 * u], 0, 0x3120);
             const uint32_t e1 = __byte_perm(a[2 * u + 1], 0, 0x3120);
-            const uint32_t w[4] = {widen_e4m3(e0), widen_e4m3(e0 >> 16), widen_e4m3(e1),
-                                   widen_e4m3(e1 >> 16)};
+            uint32_t w[4] = {widen_e4m3(e0), widen_e4m3(e0 >> 16), widen_e4m3(e1),
+                             widen_e4m3(e1 >> 16)};
             multiply(w, s + u);
           }
         }

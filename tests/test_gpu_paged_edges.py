@@ -280,3 +280,24 @@ def test_many_small_weights_behind_a_large_one(kind, cache, prompt):
     tol = (UNIT[kind] + 2.0 ** -13) * want + 4095 * 2.0 ** -32 * 256
     assert (np.abs(out - want) <= tol).all()
     assert (np.abs(lse - want_lse) <= 2.0 ** -20 * (1 + abs(want_lse))).all()
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("kind", ["bfloat16", "float16"])
+def test_infinite_values(kind, prompt):
+    """A visible infinite value makes its channel infinite, both signs make it
+    NaN, and other channels stay as they are."""
+    rng = np.random.default_rng(25)
+    k0 = rng.integers(-3, 4, 300).astype(float)
+    v0 = rng.integers(-8, 9, (300, 64)).astype(float)
+    plain, _ = attend_alike(kind, kind, k0, v0, 0.7, prompt)
+    v0[17, 3] = np.inf
+    v0[280, 4] = -np.inf
+    v0[[5, 99], 5] = np.inf
+    v0[[6, 100], 6] = np.inf, -np.inf
+    v0[250, 7] = np.nan
+    out, lse = attend_alike(kind, kind, k0, v0, 0.7, prompt)
+    assert (out[:, [3, 5]] == np.inf).all() and (out[:, 4] == -np.inf).all()
+    assert np.isnan(out[:, [6, 7]]).all()
+    assert np.array_equal(np.delete(out, range(3, 8), 1), np.delete(plain, range(3, 8), 1))
+    assert np.isfinite(lse).all()
