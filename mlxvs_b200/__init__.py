@@ -608,15 +608,10 @@ def profile_issued(kernel=None):
     return ops.value
 
 
-_PAGED = ("PagedTables", "paged_tables", "paged_store", "paged_select", "paged_attention")
-
-
-def __getattr__(name):
-    # The paged cache's functions take torch tensors only: their module, and
-    # torch with it, is imported when one of them is first used.
-    if name in _PAGED:
-        from . import paged
-
-        globals().update((n, getattr(paged, n)) for n in _PAGED)
-        return globals()[name]
-    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+from .paged import (  # noqa: E402  (needs _check and _load)
+    PagedTables,
+    paged_attention,
+    paged_select,
+    paged_store,
+    paged_tables,
+)

@@ -19,9 +19,6 @@ for the GPU, so a step of fixed sizes can be captured in a CUDA graph.
 import collections
 import struct
 
-import torch
-from torch import Tensor, float32, int8, int32, int64
-
 from . import _check, _load
 
 PagedTables = collections.namedtuple("PagedTables", "starts requests lengths slots used")
@@ -30,13 +27,25 @@ PagedTables = collections.namedtuple("PagedTables", "starts requests lengths slo
 _CACHE = struct.Struct("=QQqqqqqqqQQiiiiff")
 _QUERIES = struct.Struct("=QqqqQqqQQii")
 
-_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float8_e4m3fn: 2}
+torch = None
 
-# A decoding step makes these calls per layer, so their own time counts: the
-# checks below read each tensor's fields once, and the stream is read without
-# the Stream object that torch.cuda.current_stream builds.
-_current_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch.cuda.current_device
+
+def _ready():
+    """The library, with torch and what is used of it: the package is imported
+    without torch, which these functions need and the search does not.
+
+    A decoding step makes these calls per layer, so their own time counts: the
+    checks below read each tensor's fields once, and the stream is read without
+    the Stream object that torch.cuda.current_stream builds."""
+    if torch is None:
+        import torch as t
+
+        globals().update(
+            Tensor=t.Tensor, float32=t.float32, int8=t.int8, int32=t.int32, int64=t.int64,
+            _TYPES={t.float16: 0, t.bfloat16: 1, t.float8_e4m3fn: 2},
+            _current_stream=t._C._cuda_getCurrentRawStream,
+            _current_device=t.cuda.current_device, torch=t)
+    return _load()
 
 
 def _type(t, op, name):
@@ -160,7 +169,7 @@ def paged_tables(past, fresh, table, free_pages, page_size, num_tokens, *, strea
     tokens that got no slot (free_pages ended, or the table is too narrow).
     """
     op = "mlxvs::paged_tables"
-    lib = _load()
+    lib = _ready()
     if not (isinstance(past, Tensor) and past.is_cuda):
         raise ValueError(f"[{op}] past must be a contiguous 1-D CUDA tensor of torch.int32.")
     index = past.get_device()
@@ -201,7 +210,7 @@ def paged_store(k, v, slots, keys, values, codes=None, scales=None, *, k_scale=1
     Slots must differ, and a page's new rows be tokens in a row, one row on for
     each token; any of them may be skipped, which leaves its row as it was."""
     op = "mlxvs::paged_store"
-    lib = _load()
+    lib = _ready()
     ks = _rows(k, op, "k", _K_DIMS)
     vs = _rows(v, op, "v", _K_DIMS)
     index = k.get_device()
@@ -236,7 +245,7 @@ def paged_select(q, codes, scales, table, lengths, page_size, n, *, requests=Non
     its row of the table (None: token t has row t).
     """
     op = "mlxvs::paged_select"
-    lib = _load()
+    lib = _ready()
     n = int(n)
     queries, shape, index = _queries(q, table, lengths, requests, op)
     if stream is not None:
@@ -268,7 +277,7 @@ def paged_attention(q, keys, values, table, lengths, *, requests=None, pages=Non
     [tokens, query heads] (-inf for a token with no keys).
     """
     op = "mlxvs::paged_attention"
-    lib = _load()
+    lib = _ready()
     queries, shape, index = _queries(q, table, lengths, requests, op)
     if stream is not None:
         with _stream(stream, index):
