@@ -132,6 +132,21 @@ def _queries(q, table, lengths, requests, op):
         lengths.data_ptr(), shape[1], _type(q, op, "q")), shape, index
 
 
+def _whole(x, op, what, low=-2**31, high=2**31):
+    """A whole number that the C entries take in 32 bits (their range checks
+    would see what is left of a larger one)."""
+    x = int(x)
+    if not low <= x < high:
+        raise ValueError(f"[{op}] {what}")
+    return x
+
+
+_PAGE_SIZE = "page_size must be in [1, 1024]."
+_N = "n must be in [1, 256]."
+_ENDS = "first and last must be at least 0 and together at most n."
+_TOKENS = "num_tokens must be in [0, 2^31)."
+
+
 def _stream(stream, index):
     """A context in which `stream` (a torch stream or a cudaStream_t) is the
     current one, so that outputs are allocated in its order as well."""
@@ -170,6 +185,8 @@ def paged_tables(past, fresh, table, free_pages, page_size, num_tokens, *, strea
     """
     op = "mlxvs::paged_tables"
     lib = _ready()
+    page_size = _whole(page_size, op, _PAGE_SIZE)
+    num_tokens = _whole(num_tokens, op, _TOKENS, 0)
     if not (isinstance(past, Tensor) and past.is_cuda):
         raise ValueError(f"[{op}] past must be a contiguous 1-D CUDA tensor of torch.int32.")
     index = past.get_device()
@@ -180,18 +197,16 @@ def paged_tables(past, fresh, table, free_pages, page_size, num_tokens, *, strea
     _want(fresh, op, "fresh", int32, 1, index)
     _want(table, op, "table", int32, 2, index)
     _want(free_pages, op, "free_pages", int32, 1, index)
-    requests, num_tokens = past.shape[0], int(num_tokens)
+    requests = past.shape[0]
     rows, width = table.shape
     if fresh.shape[0] != requests or rows != requests:
         raise ValueError(f"[{op}] past, fresh and table must have one row per request.")
-    if num_tokens < 0:
-        raise ValueError(f"[{op}] num_tokens must be in [0, 2^31).")
     slots = past.new_empty(num_tokens, dtype=int64)
     ints = past.new_empty(2 * num_tokens + requests + 3)
     at = ints.data_ptr()
     starts = at + 8 * num_tokens
     _call(lib.mlxvs_paged_tables_device,
-          (past.data_ptr(), fresh.data_ptr(), requests, int(page_size), free_pages.data_ptr(),
+          (past.data_ptr(), fresh.data_ptr(), requests, page_size, free_pages.data_ptr(),
            free_pages.shape[0], table.data_ptr(), width, num_tokens, starts, at,
            at + 4 * num_tokens, slots.data_ptr(), starts + 4 * (requests + 1)), index)
     of, lengths, starts, used = torch.split_with_sizes(
@@ -246,7 +261,9 @@ def paged_select(q, codes, scales, table, lengths, page_size, n, *, requests=Non
     """
     op = "mlxvs::paged_select"
     lib = _ready()
-    n = int(n)
+    n = _whole(n, op, _N, 1, 257)
+    page_size = _whole(page_size, op, _PAGE_SIZE)
+    first, last = _whole(first, op, _ENDS), _whole(last, op, _ENDS)
     queries, shape, index = _queries(q, table, lengths, requests, op)
     if stream is not None:
         with _stream(stream, index):
@@ -258,10 +275,10 @@ def paged_select(q, codes, scales, table, lengths, page_size, n, *, requests=Non
     pages, heads = codes.shape[:2]
     _bounds(codes, scales, op, pages, heads, shape[2], index)
     cache = _CACHE.pack(0, 0, 0, 0, 0, 0, 0, 0, pages, codes.data_ptr(), scales.data_ptr(),
-                        int(page_size), heads, shape[2], _type(q, op, "q"), 1.0, 1.0)
-    out = table.new_empty((shape[0], heads, max(n, 0)))
+                        page_size, heads, shape[2], _type(q, op, "q"), 1.0, 1.0)
+    out = table.new_empty((shape[0], heads, n))
     _call(lib.mlxvs_paged_select_device,
-          (cache, queries, n, int(first), int(last), out.data_ptr()), index)
+          (cache, queries, n, first, last, out.data_ptr()), index)
     return out
 
 

@@ -4,6 +4,9 @@ import os
 import subprocess
 import sys
 
+import pytest
+
+import mlxvs_b200 as mv
 from tests.test_paged_args import AT, cache, lib, queries, refused  # noqa: F401
 
 
@@ -29,3 +32,17 @@ def test_all_names_without_torch():
             "except ValueError as e: assert 'CUDA tensor' in str(e)\n"
             "assert 'torch' in sys.modules\n")
     subprocess.run([sys.executable, "-c", code], cwd=root, check=True)
+
+
+def test_whole_numbers_past_32_bits():
+    """What is left of a larger number in 32 bits is not taken for it."""
+    wide = 2 ** 32
+    for n, kw in ((wide + 4, {}), (4, dict(page_size=wide + 16)), (4, dict(first=wide + 1)),
+                  (4, dict(last=-wide + 1)), (0, {}), (257, {})):
+        with pytest.raises(ValueError, match="must be"):
+            mv.paged_select(None, None, None, None, None, kw.pop("page_size", 16), n, **kw)
+    with pytest.raises(ValueError, match="page_size must be in"):
+        mv.paged_tables(None, None, None, None, wide + 16, 4)
+    for tokens in (-1, 2 ** 31, wide + 4):
+        with pytest.raises(ValueError, match="num_tokens must be in"):
+            mv.paged_tables(None, None, None, None, 16, tokens)
