@@ -183,15 +183,20 @@ CUtensorMap cache_map(const void* base, const AttentionParams& p, int64_t head_s
   return m;
 }
 
-// Whether selected pages are walked by tiles of tokens: prompts (more tokens
-// than requests) with enough tiles for the SMs, and a cache that a tensor map
-// can describe.  Pages of under 16 rows would leave most of a stage empty.
-// 5,229 tokens with 16 pages of 64: 672 us by tiles, 1423 by rows of their own
-// pages (10.7 GB from L2, 7.5 TB/s).
+// Whether selected pages are walked by tiles of tokens: prompts with enough
+// tiles for the SMs, and a cache that a tensor map can describe.  Pages of under
+// 16 rows would leave most of a stage empty.  A tile walks its requests one after
+// another, so it needs many tokens of each; the host knows the tokens and the
+// table's rows, idle ones among them, so what it asks for is 32 tokens a row.
+// Attention of 16 pages of 64 a token, by tiles and by rows of their own pages:
+// 400 tokens (8 key heads of 4, bf16) of 200 requests 564 and 247 us, of 50
+// requests 255 and 244, of 25 189 and 197, of one 142 and 172; 1,000 tokens (4 key
+// heads of 8) of 125 requests 328 and 305, of 31 211 and 221, of 10 195 and 221;
+// 5,229 tokens of 3 requests 768 and 1110.
 template <class T, class C, int DP>
 bool prompt_tiles(const AttentionParams& p, const DeviceInfo& dev) {
   using S = PromptShape<T, C, DP>;
-  if (p.selected == nullptr || p.tokens <= p.rows || p.page.d < 16 || p.pages == 0) return false;
+  if (p.selected == nullptr || p.tokens < 32 * p.rows || p.page.d < 16 || p.pages == 0) return false;
   const int64_t limit = (1LL << 40) / (int64_t)sizeof(C);
   for (int64_t s : {p.key_page, p.value_page})
     if (p.pages > 1 && (s == 0 || s >= limit)) return false;

@@ -141,3 +141,26 @@ def test_cut_rows_and_prompts_in_a_graph():
         check_attention(got[2], got[3], pq, keys, values, host, seen, requests, dim ** -0.5,
                         "float16", chosen)
     mv.synchronize()
+
+
+@pytest.mark.parametrize("requests,per,tiles", [(200, 2, 0), (50, 8, 0), (8, 60, 1), (1, 420, 1)])
+def test_tokens_a_request_of_the_prompt_kernel(requests, per, tiles):
+    """Steps of few tokens a request are not walked as a prompt is, and give
+    the same."""
+    rng = np.random.default_rng(requests)
+    page, heads, group, dim, length = 16, 8, 2, 64, max(100, per)
+    pages = requests * -(-length // page) + 2
+    keys, values = make_cache(rng, pages, page, heads, dim, "bfloat16")
+    table = make_table(rng, [length] * requests, page, pages)
+    rows = np.repeat(np.arange(requests), per)
+    seen = np.tile(np.arange(length - per, length) + 1, requests)
+    q = 2 * rng.standard_normal((len(rows), heads * group, dim))
+    q = torch_().from_numpy(q).cuda().to(dtype("bfloat16"))
+    chosen = lists_of_pages(rng, seen, rows, page, heads, 3)
+    mv.profile_enable()
+    out, lse = mv.paged_attention(q, keys, values, on_gpu(table), on_gpu(seen), return_lse=True,
+                                  pages=on_gpu(chosen), requests=on_gpu(rows))
+    launches = mv.profile_read("paged_prompt")[1]
+    mv.profile_enable(False)
+    assert launches == tiles
+    check_attention(out, lse, q, keys, values, table, seen, rows, dim ** -0.5, "bfloat16", chosen)
