@@ -522,7 +522,7 @@ __global__ void __launch_bounds__(AttentionShape<T, C, DP, NT>::WARPS * 32,
           }
         top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
         top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-        const int e = code_exponent(top);
+        const int e = query_exponent(top);
         const float by = exp2_int(e), back = exp2_int(-e) * p.scale;
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s)

@@ -53,6 +53,14 @@ __device__ __forceinline__ int code_exponent(float top) {
   return max(-100, min(100, 6 - floor_log2));
 }
 
+// The same for queries that go to the tensor cores as float16: kept within +-126,
+// the widest that leaves 2^e and 2^-e ordinary floats, so that neither the
+// largest bfloat16 queries overflow nor the smallest vanish.
+__device__ __forceinline__ int query_exponent(float top) {
+  const int floor_log2 = (int)((__float_as_uint(top) >> 23) & 255u) - 127;
+  return max(-126, min(126, 6 - floor_log2));
+}
+
 __device__ __forceinline__ float exp2_int(int e) {
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }

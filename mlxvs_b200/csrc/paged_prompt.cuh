@@ -333,7 +333,7 @@ __global__ void __launch_bounds__((PromptShape<T, C, DP>::WARPS + 1) * 32, 1)
           }
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-          const int e = code_exponent(top);
+          const int e = query_exponent(top);
           const float by = exp2_int(e);
           if (lane == 0) sh_factor[column][head] = exp2_int(-e) * p.scale;
 #pragma unroll

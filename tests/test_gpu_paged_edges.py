@@ -301,3 +301,32 @@ def test_infinite_values(kind, prompt):
     assert np.isnan(out[:, [6, 7]]).all()
     assert np.array_equal(np.delete(out, range(3, 8), 1), np.delete(plain, range(3, 8), 1))
     assert np.isfinite(lse).all()
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("size", [1e36, 1e-37, 2.0 ** -130])
+def test_queries_of_any_size_over_an_8_bit_cache(size, prompt):
+    """bfloat16 queries near the ends of their range, with a scale that makes
+    their scores ordinary: as those of size 1.  Powers of two and products by
+    them are exact, so only the scale's rounding is left (2^-24 of scores of at
+    most 6, twice that in a weight)."""
+    torch = torch_()
+    rng = np.random.default_rng(26)
+    page, heads, dim, length = 64, 8, 64, 300
+    keys, values = make_cache(rng, 5, page, heads, dim, "float8_e4m3fn")
+    tokens, rows = (600, 1) if prompt else (64, 64)
+    q = torch.from_numpy(rng.integers(-3, 4, (tokens, heads, dim))).cuda().bfloat16()
+    by = 2.0 ** np.floor(np.log2(size))  # exact, for subnormal ones as well
+    table = on_gpu(np.arange(5)[None].repeat(rows, 0))
+    more = {}
+    if prompt:
+        more = dict(requests=on_gpu([0] * tokens),
+                    pages=on_gpu(np.arange(5)).expand(tokens, heads, -1).contiguous())
+    lengths = on_gpu([length] * tokens)
+    want, want_lse = mv.paged_attention(q, keys, values, table, lengths, scale=1 / 32,
+                                        return_lse=True, **more)
+    out, lse = mv.paged_attention((q.double() * by).bfloat16(), keys, values, table, lengths,
+                                  scale=1 / 32 / by, return_lse=True, **more)
+    assert np.isfinite(wide(out)).all()
+    assert (np.abs(wide(lse) - wide(want_lse)) <= 2.0 ** -20 * (1 + np.abs(wide(want_lse)))).all()
+    assert (np.abs(wide(out) - wide(want)) <= 2 * UNIT["bfloat16"] * np.abs(wide(want)) + 1e-5).all()
