@@ -283,6 +283,11 @@ void paged_store(const mlxvs_paged_cache& c, const void* k, const void* v, int t
   for (int64_t x : {k_head, v_head})
     REQUIRE(c.heads <= 1 || (x >= 0 && x % 8 == 0),
             "the strides of k and v must be multiples of 16 bytes.");
+  // rows that share memory would be written by several blocks at a time
+  REQUIRE((c.pages <= 1 || (c.key_page_stride > 0 && c.value_page_stride > 0)) &&
+              (c.page_size <= 1 || (c.key_row_stride > 0 && c.value_row_stride > 0)) &&
+              (c.heads <= 1 || (c.key_head_stride > 0 && c.value_head_stride > 0)),
+          "the cache's rows must lie apart: strides of 0 can only be read.");
   if (c.codes != nullptr || c.scales != nullptr) check_codes(op, c);
   DeviceInfo& dev = device_info();
   if (tokens == 0 || c.pages == 0) return;

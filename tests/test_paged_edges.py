@@ -80,3 +80,11 @@ def test_struct_fields_lie_where_the_header_has_them(tmp_path):
         for i, (offset, width) in enumerate(zip(pairs[::2], pairs[1::2])):
             assert offset == struct.calcsize("=" + kinds[:i]), fields[i]
             assert width == struct.calcsize("=" + kinds[i]), fields[i]
+
+
+@pytest.mark.parametrize("stride", ["kp", "kr", "kh", "vp", "vr", "vh"])
+def test_store_into_rows_that_share_memory(lib, stride):  # noqa: F811
+    """A cache with a stride of 0 can be read, not written."""
+    c = cache(**{stride: 0})
+    refused(lib, lib.mlxvs_paged_store_device(c, AT, AT, 1, 3, 256, 128, 256, 128, AT, None),
+            "must lie apart")
