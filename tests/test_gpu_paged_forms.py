@@ -164,3 +164,30 @@ def test_tokens_a_request_of_the_prompt_kernel(requests, per, tiles):
     mv.profile_enable(False)
     assert launches == tiles
     check_attention(out, lse, q, keys, values, table, seen, rows, dim ** -0.5, "bfloat16", chosen)
+
+
+@pytest.mark.parametrize("heads,group,page,tokens,length,kind,cache", [
+    (1, 2, 16, 3400, 3500, "bfloat16", "bfloat16"),
+    (1, 1, 64, 3300, 3300, "float16", "float8_e4m3fn"),
+    (8, 2, 1024, 700, 900, "float16", "float16"),  # one page
+])
+def test_prompts_over_dimensions_of_one(heads, group, page, tokens, length, kind, cache):
+    """One key head, or one page: such a dimension's stride may be any."""
+    rng = np.random.default_rng(page)
+    dim, pages = 64, -(-length // page)
+    keys, values = make_cache(rng, pages, page, heads, dim, cache)
+    strides = list(keys.stride())
+    strides[2 if heads == 1 else 0] = 7
+    odd = [x.as_strided(x.shape, strides) for x in (keys, values)]
+    table = make_table(rng, [length], page, pages)
+    rows, seen = [0] * tokens, np.arange(length - tokens, length) + 1
+    q = 2 * rng.standard_normal((tokens, heads * group, dim))
+    q = torch_().from_numpy(q).cuda().to(dtype(kind))
+    chosen = lists_of_pages(rng, seen, rows, page, heads, 6)
+    mv.profile_enable()
+    out, lse = mv.paged_attention(q, *odd, on_gpu(table), on_gpu(seen), return_lse=True,
+                                  pages=on_gpu(chosen), requests=on_gpu(rows))
+    launches = mv.profile_read("paged_prompt")[1]
+    mv.profile_enable(False)
+    assert launches == 1
+    check_attention(out, lse, q, keys, values, table, seen, rows, dim ** -0.5, kind, chosen)
