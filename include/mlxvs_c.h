@@ -362,8 +362,9 @@ typedef enum {
   MLXVS_FLOAT8_E4M3 = 2,
 } mlxvs_dtype;
 
-/** A cache's tensors; strides in elements, multiples of 16 bytes; the head
- * dimension is contiguous, a multiple of 16 bytes and at most 256. */
+/** A cache's tensors; strides in elements, multiples of 16 bytes (0 where the
+ * cache is only read); the head dimension is contiguous, a multiple of 16 bytes
+ * and at most 256. */
 typedef struct {
   void* keys;
   void* values;
@@ -372,7 +373,10 @@ typedef struct {
   int64_t pages;
   /** Bounds of the pages' keys, int8 [pages, heads, 2, dim] and float32
    * [pages, heads], in the cache's units: codes[.., 0, d] * scale <= key[d]
-   * <= codes[.., 1, d] * scale.  May be NULL where no pages are selected. */
+   * <= codes[.., 1, d] * scale, but that codes end at -127 and 127: where the
+   * page's largest magnitude is within a step of 128 steps the bound is short by
+   * up to that step, and keys of 2^107 and more are not bounded.  May be NULL
+   * where no pages are selected. */
   int8_t* codes;
   float* scales;
   int32_t page_size;
@@ -406,7 +410,8 @@ typedef struct {
  * its row of table [requests, width] lists are taken from free_pages, in
  * request order, and entered in the table.  Per new token t of num_tokens
  * (at least their number; the tokens past it are padding, so that a
- * captured step can keep its size): token_requests (-1 for padding), lengths
+ * captured step can keep its size; with fewer, the last tokens get nothing):
+ * token_requests (-1 for padding), lengths
  * (the token's position + 1: the keys it sees; 0 for padding) and slots
  * (page * page_size + row in the page, -1 where it gets none).  Lengths and
  * the sum of fresh must stay below 2^31.  starts
@@ -461,10 +466,12 @@ MLXVS_C_API int mlxvs_paged_store_device(
  * that each token and key head attends to: pages int32 [tokens, heads, n] in
  * ascending order, -1 past the last.  All pages that hold keys of the token
  * when they are at most n; else the first `first` and last `last` of them and
- * those of the best scores, ties to the lower page.  A page's score is an
- * 8-bit upper bound of q . key over its rows, summed over the query heads of
- * the key head, from the cache's codes and scales (keys and values are not
- * read); it is exact in float32, so the choice is the same on every run.
+ * those of the best scores, ties to the lower page, NaN scores last.  A page's
+ * score is an 8-bit estimate of the upper bound of q . key over its rows, summed
+ * over the query heads of the key head, from the cache's codes and scales (keys
+ * and values are not read): the queries' codes are rounded to nearest and their
+ * sum over the heads is cut to 7 bits, so it can lie a little below the bound.
+ * It is exact in float32, so the choice is the same on every run.
  */
 MLXVS_C_API int mlxvs_paged_select_device(
     const mlxvs_paged_cache* cache,

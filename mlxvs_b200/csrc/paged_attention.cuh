@@ -13,10 +13,15 @@
 // sum, weighted values) that a second kernel joins in the order of the keys.
 //
 // Measured, with the joining kernel: 64 requests of 0 to 5,000 keys (bf16, 8 key
-// heads of 4) 66 us, 5.7 TB/s; 200 requests of up to 16,000 keys (f16, 4 key heads
-// of 16) 395 us, 6.7 TB/s, the rate of a copy; 3 requests of up to 200,001 keys in
-// e4m3 (8 key heads of 8) 168 us, 5.5 TB/s, where the warps' conversions and the
-// short ring show.
+// heads of 4) 67 us, 5.7 TB/s; 200 requests of up to 16,000 keys (f16, 4 key heads
+// of 16) 405 us, 6.5 TB/s, the rate of a copy, and up to 455 where the power limit
+// lowers the clock; 3 requests of up to 200,001 keys in e4m3 (8 key heads of 8) 171
+// us, 5.4 TB/s, where the warps' conversions and the short ring show.
+//
+// Several tokens of a request are rows of their own, each of which reads the keys
+// again: 2,048 tokens that see up to 12,000 keys (bf16, 4 key heads of 8) take 3.7
+// ms, 17 times their operations' floor (e4m3 3.1 ms); 64 requests of 4 tokens and
+// 8,000 keys 603 us against 161 for the bytes (e4m3 324 against 81).
 #pragma once
 
 #include <type_traits>
@@ -217,8 +222,9 @@ struct AttentionShape {
   // leaves each: three blocks with rings of two steps against two with three took
   // 166 for 175 us on long 8-bit caches, and 20 for 23 us on short lists of pages
   // (the products' latency counts there), the same on others.  Rows of 512 bytes:
-  // two blocks of three warps against one of four 140 for 182 us (8 requests up
-  // to 112,749 keys, 16 heads a key head).
+  // two blocks of three warps against one of four 149 for 197 us (8 requests up
+  // to 112,749 keys, 2 key heads of 16, bf16; the kernel alone).  There the sums'
+  // compensation costs 8 us in registers.
   static constexpr int WARPS = STEP > 8192 ? 3 : 4;
   static constexpr int BLOCKS = STEP <= 8192 && NT == 1 && DP <= 128 ? 3 : 2;
   static constexpr int STAGES =

@@ -12,7 +12,9 @@
 // work is spent on tokens that did not select the page.
 //
 // Bound: 5,229 tokens with 16 of up to 230 pages of 64 each (bf16, 4 key heads of
-// 8, 89 GFLOP) take 672 us, 133 TFLOP/s.  Parts switched off in turn: the loads
+// 8, 89 GFLOP) take 693 us, 128 TFLOP/s, and 799 over an e4m3 cache.  Parts switched
+// off in turn when they took 672 (without the care for infinite values and small
+// weights): the loads
 // alone take 298 us (the tiles still read 2.5 GB from L2) and hide behind the
 // products, which alone take 635; of those the waits for the slowest warp of a
 // stage cost 76, the scores 224, the weights 69, the values 171 and the lists and
@@ -99,8 +101,8 @@ __device__ __forceinline__ void prompt_keys(float (&o)[DP / 16][NT][4], float (&
     for (int nt = 0; nt < NT; ++nt)
       st[mt][nt][0] = st[mt][nt][1] = st[mt][nt][2] = st[mt][nt][3] = 0.0f;
   // A loop over an 8-bit cache's steps, for which the widening makes the bodies
-  // twice as long: 5,229 tokens' prompt 1,064 us unrolled, 856 rolled (a 16-bit
-  // cache's 748 and 815).
+  // twice as long: 5,229 tokens and their selection 1,064 us unrolled, 856 rolled
+  // (a 16-bit cache's 748 and 815).
 #pragma unroll(S::EIGHT ? 1 : DP / 32)
   for (int s = 0; s < DP / 16; s += 2) {
     uint32_t q[NT][4];  // operands of steps s and s + 1

@@ -1,14 +1,15 @@
 // Page selection: the n pages of its request that each new token and key
 // head attends to.
 //
-// The score of a page is an upper bound of q . key over its rows, summed over
-// the query heads of the key head, in 8 bits: with the page's bounds lo, hi
-// and the parts q+ = max(q, 0), q- = min(q, 0),
+// The score of a page is an estimate in 8 bits of the upper bound of q . key over
+// its rows, summed over the query heads of the key head: with the page's bounds
+// lo, hi and the parts q+ = max(q, 0), q- = min(q, 0),
 //     q . key <= q+ . hi + q- . lo   for every key of the page.
 // The query heads share one power of two that puts their largest magnitude in
 // [64, 128); each is rounded to whole numbers of at most 127, the parts are
 // summed over the heads and shifted right by ceil(log2 G), which leaves codes
-// of at most 127.  The dot products are whole numbers below 2^24
+// of at most 127: rounding to nearest and the shift can leave a score a little
+// below the bound.  The dot products are whole numbers below 2^24
 // (2 * 256 * 127 * 127 at the widest), the page's scale is a power of two, so
 // a score is one exact float: it does not depend on the order of the sums,
 // and ties (to the lower page) are real ties.
@@ -192,8 +193,8 @@ __device__ __forceinline__ void select_pages(const uint32_t* keys, int held, int
 // many blocks per SM: fetching the codes a step ahead as well took 143
 // registers and made prompts of 5,229 tokens slower (97 -> 144 us).  Now those
 // take 56 us (8 to start, 18 for the query codes, 14 for the scores, 16 for the
-// selection), 32 single tokens with up to 500 pages 11 us, and 7 with up to 3,900
-// pages (27 MB of codes) 21 us, of which 9 for the scores and 8 for the selection.
+// selection), 32 single tokens with up to 500 pages 11.5 us, and 7 with up to 3,900
+// pages (27 MB of codes) 21.5 us, of which 9 for the scores and 8 for the selection.
 //
 // SEG: 64-byte segments of a page's codes (dim up to 32 SEG).
 template <class T, int TT, int SEG>

@@ -11,9 +11,10 @@
 // request, from L2) and keeps those that its own range of tokens meets.  One
 // launch; the work is 16 bytes written per token.
 //
-// Bound: the latency of lengths -> sums -> pages -> slots.  64 requests with a
-// token each take 3.2 us; 1,000 requests with 665,693 new tokens 8.8 us (1.2
-// TB/s; the floor at the copy rate is 1.6 us, at a launch's latency 3).
+// Bound: the latency of lengths -> sums -> pages -> slots, and for prompts the
+// instructions of each token's search and division (issue slots 52 % busy).  64
+// requests with a token each take 3.1 us; 1,000 requests with 665,693 new tokens
+// 8.6 us (1.2 TB/s; the floor at the copy rate is 1.6 us, at a launch's latency 3).
 #pragma once
 
 #include "paged_common.cuh"

@@ -13,7 +13,8 @@ pages are to be selected, codes int8 [pages, key heads, 2, dim] and scales
 float32 [pages, key heads]: bounds of each page's keys.  table int32
 [requests, width] lists each request's pages in order.  Calls are queued on
 the current stream (or `stream=`), allocate their outputs only, and never wait
-for the GPU, so a step of fixed sizes can be captured in a CUDA graph.
+for the GPU, so a step of fixed sizes can be captured in a CUDA graph.  They are
+for inference: results carry no gradients, whatever their inputs do.
 """
 
 import collections
@@ -249,8 +250,8 @@ def paged_store(k, v, slots, keys, values, codes=None, scales=None, *, k_scale=1
 
 def paged_select(q, codes, scales, table, lengths, page_size, n, *, requests=None, first=1,
                  last=1, stream=None):
-    """The n pages that each token and key head attends to, by an 8-bit bound
-    of its scores: int32 [tokens, key heads, n], positions in the request's
+    """The n pages that each token and key head attends to, by an 8-bit estimate
+    of the bound of its scores: int32 [tokens, key heads, n], positions in the request's
     row of table, ascending, -1 past the last.  The first `first` and last
     `last` pages that hold keys of the token are always among them; ties go to
     the lower page.
@@ -285,8 +286,9 @@ def paged_select(q, codes, scales, table, lengths, page_size, n, *, requests=Non
 def paged_attention(q, keys, values, table, lengths, *, requests=None, pages=None, scale=None,
                     k_scale=1.0, v_scale=1.0, return_lse=False, stream=None):
     """Attention of each token over its request's first `lengths` keys, or over
-    those of them in the pages that paged_select lists for it: softmax(scale *
-    q . k) v, of q's shape and type.  scale: 1 / sqrt(dim) by default.  Query
+    those of them in the pages that paged_select lists for it (a page at most
+    once for a token and key head): softmax(scale * q . k) v, of q's shape and
+    type.  scale: 1 / sqrt(dim) by default.  Query
     head i reads key head i // (query heads // key heads).  A token with no
     keys gets zeros.
 
